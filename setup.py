@@ -64,8 +64,8 @@ def _hipcc_ext(name, sources, out_dir, extra_link=()):
         src_path = os.path.join(ROOT, src)
         import glob
 
-        deps = [src_path] + glob.glob(os.path.join(ROOT, "csrc", "**",
-                                                   "*.h*"), recursive=True)
+        deps = [src_path, os.path.abspath(__file__)] + glob.glob(
+            os.path.join(ROOT, "csrc", "**", "*.h*"), recursive=True)
         if (os.path.exists(obj) and
                 os.path.getmtime(obj) > max(map(os.path.getmtime, deps))):
             objs.append(obj)
@@ -74,6 +74,8 @@ def _hipcc_ext(name, sources, out_dir, extra_link=()):
             HIPCC, "-c", src_path, "-o", obj,
             f"--offload-arch={HIP_ARCH}", "-O3", "-std=c++17", "-fPIC",
             f"-I{py_inc}", f"-I{pb_inc}", "-I/opt/rocm/include",
+            # no packed f32 arithmetic (v_pk_*_f32) in device code
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         ]
         print("+", " ".join(cmd))
         subprocess.check_call(cmd)
