@@ -51,6 +51,21 @@ hipError_t kf_ln_fwd(const void *, void *, const void *, const void *,
 hipError_t kf_ln_bwd(const void *, const void *, const void *, const void *,
                      const void *, long long, int, void *, void *, void *);
 hipError_t kf_ln_fold(void *, int, void *);
+size_t kf_embed_ws(long long, long long, int);
+hipError_t kf_embed_fwd(const void *, int, const void *, long long, int,
+                        void *, int, long long, long long, int, float,
+                        void *);
+hipError_t kf_embed_bwd(const void *, int, const void *, int, void *, int,
+                        long long, long long, int, long long, float, void *,
+                        void *);
+long long kf_qk_ws(int);
+hipError_t kf_qk_norm_rope(const uintptr_t *, const long long *, int, float,
+                           int, void *);
+long long kf_attn_ws(const long long *, int);
+hipError_t kf_attn_fwd(const uintptr_t *, const long long *,
+                       const long long *, float, int, void *);
+hipError_t kf_attn_bwd(const uintptr_t *, const long long *,
+                       const long long *, float, int, void *);
 }
 
 namespace {
@@ -62,6 +77,18 @@ void check(hipError_t e, const char *what)
                                  hipGetErrorString(e));
     }
 }
+
+// Lists cross from Python as vectors; the kernels' entries read a fixed
+// number of each.
+template <typename T>
+const T *list(const std::vector<T> &v, size_t n, const char *what)
+{
+    if (v.size() != n)
+        throw std::invalid_argument(std::string(what) + ": wrong list");
+    return v.data();
+}
+typedef std::vector<uintptr_t> Ptrs;
+typedef std::vector<long long> Dims;
 
 struct ChunkHost {
     const void *src;
@@ -272,6 +299,66 @@ PYBIND11_MODULE(_hip, m)
     m.def("ln_fold", [](uintptr_t wb, int H, uintptr_t stream) {
         check(kf_ln_fold((void *)wb, H, (void *)stream), "kf_ln_fold");
     });
+
+    // ---- embedding lookup with a scale, gradient by sorted tokens ----
+    m.def("embed_ws", [](long long N, long long V, int H) {
+        return (long long)kf_embed_ws(N, V, H);
+    });
+    m.def("embed_fwd",
+          [](uintptr_t ids, bool wide, uintptr_t w, long long ldw, int wtype,
+             uintptr_t out, int otype, long long N, long long V, int H,
+             float scale, uintptr_t stream) {
+              check(kf_embed_fwd((const void *)ids, wide ? 1 : 0,
+                                 (const void *)w, ldw, wtype, (void *)out,
+                                 otype, N, V, H, scale, (void *)stream),
+                    "kf_embed_fwd");
+          });
+    m.def("embed_bwd",
+          [](uintptr_t ids, bool wide, uintptr_t dout, int otype,
+             uintptr_t dw, int wtype, long long N, long long V, int H,
+             long long padding, float scale, uintptr_t work,
+             uintptr_t stream) {
+              check(kf_embed_bwd((const void *)ids, wide ? 1 : 0,
+                                 (const void *)dout, otype, (void *)dw,
+                                 wtype, N, V, H, padding, scale,
+                                 (void *)work, (void *)stream),
+                    "kf_embed_bwd");
+          });
+
+    // ---- query/key norm for each head with the position rotation ----
+    m.def("qk_ws", [](int D) { return kf_qk_ws(D); });
+    m.def("qk_norm_rope",
+          [](const Ptrs &ptrs, const Dims &dims, int dtype, float eps,
+             bool backward, uintptr_t stream) {
+              check(kf_qk_norm_rope(
+                        list(ptrs, backward ? 13 : 8, "qk_norm_rope"),
+                        list(dims, backward ? 23 : 17, "qk_norm_rope"),
+                        dtype, eps, backward ? 1 : 0, (void *)stream),
+                    "kf_qk_norm_rope");
+          });
+
+    // ---- attention with a sliding window and first tokens ----
+    m.def("attn_ws", [](const Dims &dims, bool backward) {
+        return kf_attn_ws(list(dims, 9, "attn_ws"), backward ? 1 : 0);
+    });
+    m.def("attn_fwd",
+          [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
+             float scale, int dtype, uintptr_t stream) {
+              check(kf_attn_fwd(list(ptrs, 8, "attn_fwd"),
+                                list(dims, 9, "attn_fwd"),
+                                list(strides, 9, "attn_fwd"), scale, dtype,
+                                (void *)stream),
+                    "kf_attn_fwd");
+          });
+    m.def("attn_bwd",
+          [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
+             float scale, int dtype, uintptr_t stream) {
+              check(kf_attn_bwd(list(ptrs, 12, "attn_bwd"),
+                                list(dims, 9, "attn_bwd"),
+                                list(strides, 12, "attn_bwd"), scale, dtype,
+                                (void *)stream),
+                    "kf_attn_bwd");
+          });
 
     // ---- fused BatchNorm(+residual+ReLU), NHWC bf16 ----
     m.def("bn_stats",

@@ -1,0 +1,1112 @@
+// Attention with a sliding window and first tokens that stay visible,
+// forward and backward — gfx950.
+//
+//   out = softmax(scale * q k^T over the visible keys) v
+// A query at position p of a sequence of n keys sees key j when j < n and
+// (|p - j| < window or j < sinks), and j <= p where causal. A query whose
+// position is outside [0, n) sees nothing: its output and gradients are 0.
+//
+// The G query heads that share a key head are flattened with the queries:
+// row r of a key head is query r / G, head r % G. Positions grow with r,
+// so a block of rows is a block of neighbouring queries, and one pass over
+// the keys serves the whole group.
+//
+// All three kernels keep one operand of 32 columns per wave in registers
+// and stream tiles of the others through LDS. Scores are computed as
+// S^T = K Q^T (forward, dq; a column is a query) or S = Q K^T (dk, dv; a
+// column is a key), with mfma 32x32x16: lane l holds column l % 32 and,
+// in accumulator r, row 8 (r / 4) + 4 (l / 32) + r % 4. The second
+// product contracts over those rows, and any order of the contracted
+// index will do as long as both operands share it: eight accumulators,
+// rounded to 16 bits, are the B operand as they are, and the A operand is
+// read from the same LDS tile by the transposing 64-bit read with the rows
+// in that order. No probability passes through LDS or between lanes.
+//
+// The backward computes the scores twice, once for dq and once for dk and
+// dv, instead of adding dq with atomics: every output is written once by
+// one block in a fixed order, so results repeat bit by bit.
+//
+// Probabilities and their gradients are rounded to the inputs' 16 bits as
+// operands of the second product (their relative error of half a step is
+// that of the inputs themselves); scores, softmax statistics, sums and
+// accumulators are f32.
+#include <climits>
+
+#include "vec.hpp"
+
+using namespace kfv;
+
+namespace {
+
+constexpr int KT = 64;  // rows of a streamed tile
+
+struct Args {
+    const void *q, *k, *v, *dout, *o;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;  // [B][Hk][S * G]; lse in powers of two
+    long long qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
+    int B, S, T, Hk, G, D;
+    int window, sinks, causal;
+    const int *lengths, *starts;
+    float scale, c;  // c = scale * log2(e)
+    int blocks;      // row blocks (or key blocks) of a key head
+    int splits;
+    float *part_o, *part_ml;     // forward, split over keys
+    float *part_k, *part_v;      // dk, dv, split over rows
+    int sink_blocks, sink_splits, splits_rows;
+};
+
+template <typename T>
+__device__ inline f32x16 mfma(s16x8 a, s16x8 b, f32x16 c);
+template <>
+__device__ inline f32x16 mfma<__bf16>(s16x8 a, s16x8 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+        0, 0);
+}
+template <>
+__device__ inline f32x16 mfma<_Float16>(s16x8 a, s16x8 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+        0);
+}
+
+// Eight accumulators, from `at`, as a 16-bit operand.
+template <typename T>
+__device__ inline s16x8 pack8(const f32x16 &x, int at)
+{
+    typename vec8<T>::type v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)x[at + i];
+    return __builtin_bit_cast(s16x8, v);
+}
+
+// LDS tile: KT rows of DP elements, rows 16 bytes apart from a power of
+// two so that neighbouring rows start in other banks.
+template <int DP>
+struct Tile {
+    static constexpr int LD = DP + 8;
+    __align__(16) short x[KT * LD];
+};
+
+// A operand from rows r0..r0+31 as they lie: row r0 + l % 32, elements
+// 16 ks + 8 (l / 32) + 0..7.
+template <int DP>
+__device__ inline s16x8 rows_op(const Tile<DP> &t, int r0, int ks, int lane)
+{
+    return *(const s16x8 *)&t.x[(r0 + lane % 32) * Tile<DP>::LD + ks * 16 +
+                                lane / 32 * 8];
+}
+
+// A operand of the transposed tile: row (of the operand) = element
+// 32 dt + l % 32, contracted index = tile rows r0 + 4 (l / 32) + 0..3 and
+// 8 rows on, the order in which the accumulators hold them.
+template <int DP>
+__device__ inline s16x8 cols_op(const Tile<DP> &t, int r0, int dt, int lane)
+{
+    const int i = lane % 16;
+    const short *p = &t.x[(r0 + lane / 32 * 4 + i / 4) * Tile<DP>::LD +
+                          dt * 32 + lane / 16 % 2 * 16 + i % 4 * 4];
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4 *)(p + 8 * Tile<DP>::LD));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A tile on its way from memory to LDS, NT threads.
+template <int DP, int NT>
+struct Stage {
+    static constexpr int N = KT * DP / 8 / NT;
+    s16x8 r[N];
+    // rows j0.. of a [T][D] matrix; rows outside [0, end) are zeros
+    __device__ void load(const void *base, long long stride, int j0, int end,
+                         int D)
+    {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int slot = threadIdx.x + v * NT;
+            const int row = slot / (DP / 8), c = slot % (DP / 8) * 8;
+            const int j = j0 + row;
+            s16x8 x = {};
+            if (j < end && c < D)
+                x = *(const s16x8 *)((const short *)base + j * stride + c);
+            r[v] = x;
+        }
+    }
+    __device__ void store(Tile<DP> &t) const
+    {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int slot = threadIdx.x + v * NT;
+            const int row = slot / (DP / 8), c = slot % (DP / 8) * 8;
+            *(s16x8 *)&t.x[row * Tile<DP>::LD + c] = r[v];
+        }
+    }
+};
+
+struct Seq {
+    int n;      // keys
+    int start;  // position of query 0
+};
+
+__device__ inline Seq sequence(const Args &a, int b)
+{
+    Seq s;
+    s.n = a.T;
+    s.start = a.T - a.S;
+    if (a.lengths) {
+        const int n = a.lengths[b];
+        s.n = n < 0 ? 0 : n > a.T ? a.T : n;
+    }
+    if (a.starts) {
+        const int p = a.starts[b];
+        const int most = 1 << 30;
+        s.start = p < -most ? -most : p > most ? most : p;
+    }
+    return s;
+}
+
+// What one query sees: keys [lo, hi] and [0, first).
+struct View {
+    int lo, hi, first;
+    __device__ bool sees(int j) const
+    {
+        return (j >= lo && j <= hi) || j < first;
+    }
+};
+
+__device__ inline View view_of(const Args &a, const Seq &s, int p)
+{
+    View v = {0, -1, 0};
+    if (p >= 0 && p < s.n) {
+        const int last = a.causal ? p : s.n - 1;
+        v.lo = p - a.window + 1;
+        v.hi = a.causal || a.window > last - p ? last : p + a.window - 1;
+        v.first = a.sinks < last + 1 ? a.sinks : last + 1;
+    }
+    return v;
+}
+
+// Tiles of keys that rows at positions p0..p1 (inside the sequence) see:
+// `head` tiles from key 0, then those from tile `from` up to `to`.
+struct Tiles {
+    int head, from, to;
+    __device__ int count() const { return head + to - from; }
+    __device__ int at(int i) const { return i < head ? i : from + i - head; }
+};
+
+__device__ inline Tiles tiles_of(const Args &a, const Seq &s, int p0, int p1)
+{
+    Tiles t = {0, 0, 0};
+    if (p0 < 0) p0 = 0;
+    if (p1 > s.n - 1) p1 = s.n - 1;
+    if (p0 > p1) return t;
+    const View x = view_of(a, s, p0), y = view_of(a, s, p1);
+    const int lo = x.lo < 0 ? 0 : x.lo;
+    int hi = y.hi + 1;
+    if (y.first > hi) hi = y.first;
+    t.from = lo / KT;
+    t.to = (hi + KT - 1) / KT;
+    const int sinks = (y.first + KT - 1) / KT;
+    t.head = sinks < t.from ? sinks : t.from;
+    return t;
+}
+
+// Whether keys k0..k1 are all seen (2), partly (1) or not at all (0) by
+// all queries of positions p0..p1.
+__device__ inline int seen(const Args &a, const Seq &s, int p0, int p1,
+                           int k0, int k1)
+{
+    if (p0 < 0) p0 = 0;
+    if (p1 > s.n - 1) p1 = s.n - 1;
+    if (p0 > p1 || k0 >= s.n) return 0;
+    const View x = view_of(a, s, p0), y = view_of(a, s, p1);
+    // the union of the windows is [x.lo, y.hi], their common part
+    // [y.lo, x.hi]; first tokens grow with p where causal
+    if (k0 >= y.first && (k0 > y.hi || k1 < x.lo)) return 0;
+    if ((k0 >= y.lo && k1 <= x.hi) || k1 < x.first) return 2;
+    return 1;
+}
+
+// Neighbouring block ids run on different XCDs; give each XCD a
+// contiguous range of the work, so that blocks of one head share an L2.
+__device__ inline unsigned work_id()
+{
+    const unsigned n = gridDim.x / 8, id = blockIdx.x;
+    return id < n * 8 ? id % 8 * n + id / 8 : id;
+}
+
+// ---- forward ----
+// A wave owns 32 rows. SPLIT: the block takes one of `splits` parts of the
+// row block's tiles and writes the sums as they are, for attn_join.
+template <typename T, int DP, int NW, bool SPLIT>
+__global__ __launch_bounds__(NW *WAVE) void attn_fwd(const Args a)
+{
+    __shared__ Tile<DP> kt, vt;
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    unsigned id = work_id();
+    int split = 0;
+    if (SPLIT) {
+        split = id % a.splits;
+        id /= a.splits;
+    }
+    const int bh = id / a.blocks;
+    // later rows see more where causal: they go first
+    const int blk = a.blocks - 1 - (int)(id - (unsigned)bh * a.blocks);
+    const int b = bh / a.Hk, h = bh - b * a.Hk;
+    const int SG = a.S * a.G;
+    const Seq s = sequence(a, b);
+
+    const int r0 = blk * NW * 32, w0 = r0 + wid * 32;
+    const int rlast = r0 + NW * 32 < SG ? r0 + NW * 32 - 1 : SG - 1;
+    const int wlast = w0 + 31 < SG ? w0 + 31 : SG - 1;
+    const int r = w0 + lane % 32, qi = r / a.G, g = r - qi * a.G;
+    const int p = s.start + qi;
+    const View view =
+        r < SG ? view_of(a, s, p) : View{0, -1, 0};
+    const bool live = r < SG && p >= 0 && p < s.n;
+    // positions of this wave's rows; none where it has no rows
+    const int wp0 = s.start + w0 / a.G;
+    const int wp1 = w0 < SG ? s.start + wlast / a.G : INT_MIN / 2;
+
+    s16x8 qop[DP / 16];
+    {
+        const short *row = (const short *)a.q + b * a.qb + qi * a.qs +
+                           (long long)(h * a.G + g) * a.qh;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int d = i * 16 + lane / 32 * 8;
+            s16x8 x = {};
+            if (live && d < a.D) x = *(const s16x8 *)(row + d);
+            qop[i] = x;
+        }
+    }
+
+    const Tiles tl =
+        tiles_of(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
+    int i = 0, end = tl.count();
+    if (SPLIT) {
+        const int n = end;
+        i = (int)((long long)n * split / a.splits);
+        end = (int)((long long)n * (split + 1) / a.splits);
+    }
+    const short *kbase = (const short *)a.k + b * a.kb + h * a.kh;
+    const short *vbase = (const short *)a.v + b * a.vb + h * a.vh;
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+    float m = -__builtin_inff(), l = 0.f;
+
+    Stage<DP, NW * WAVE> ks, vs;
+    if (i < end) {
+        ks.load(kbase, a.ks, tl.at(i) * KT, s.n, a.D);
+        vs.load(vbase, a.vs, tl.at(i) * KT, s.n, a.D);
+    }
+    for (; i < end; ++i) {
+        const int k0 = tl.at(i) * KT;
+        __syncthreads();
+        ks.store(kt);
+        vs.store(vt);
+        __syncthreads();
+        if (i + 1 < end) {
+            ks.load(kbase, a.ks, tl.at(i + 1) * KT, s.n, a.D);
+            vs.load(vbase, a.vs, tl.at(i + 1) * KT, s.n, a.D);
+        }
+        const int see = seen(a, s, wp0, wp1, k0, k0 + KT - 1);
+        if (see == 0) continue;
+        f32x16 x[KT / 32];
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+            x[t] = f32x16{};
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                x[t] = mfma<T>(rows_op<DP>(kt, t * 32, d, lane), qop[d],
+                               x[t]);
+        }
+        if (see == 1) {
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = k0 + t * 32 + e / 4 * 8 + lane / 32 * 4 +
+                                  e % 4;
+                    if (!view.sees(j)) x[t][e] = -__builtin_inff();
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m, top);
+        // a row that has seen nothing yet keeps zeros: exp2(-inf - 0)
+        const float base = mn == -__builtin_inff() ? 0.f : mn * a.c;
+        const float alpha = __builtin_amdgcn_exp2f(m * a.c - base);
+        m = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[t][e] = __builtin_amdgcn_exp2f(x[t][e] * a.c - base);
+                sum += x[t][e];
+            }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            const s16x8 pop = pack8<T>(x[t / 2], t % 2 * 8);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                o[d] = mfma<T>(cols_op<DP>(vt, t * 16, d, lane), pop, o[d]);
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (r >= SG) return;
+    if (!live) {  // a tile that its neighbours see whole is not masked
+        m = -__builtin_inff();
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+    }
+    const long long row = (long long)bh * SG + r;
+    if (SPLIT) {
+        // rows of a head in order, parts of a row together
+        float *po = a.part_o + (row * a.splits + split) * DP;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f32x4 y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = o[d][e * 4 + j];
+                *(f32x4 *)(po + d * 32 + e * 8 + lane / 32 * 4) = y;
+            }
+        if (lane < 32) {
+            float *ml = a.part_ml + (row * a.splits + split) * 2;
+            ml[0] = m * a.c;
+            ml[1] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    T *out = (T *)a.out +
+             (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c0 = d * 32 + e * 8 + lane / 32 * 4;
+            typedef __attribute__((ext_vector_type(4))) T T4;
+            T4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = (T)(o[d][e * 4 + j] * inv);
+            if (c0 < a.D) *(T4 *)(out + c0) = y;
+        }
+    // a row that sees nothing has no weight anywhere: exp2(s - inf) = 0
+    if (a.lse && lane < 32)
+        a.lse[row] = l == 0.f ? __builtin_inff() : m * a.c + log2f(l);
+}
+
+// Joins the parts of a row: one wave a row, DP / 64 columns a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
+{
+    const int lane = threadIdx.x % WAVE;
+    const int SG = a.S * a.G;
+    const long long row = (long long)blockIdx.x * 4 + threadIdx.x / WAVE;
+    if (row >= (long long)a.B * a.Hk * SG) return;
+    const float *ml = a.part_ml + row * a.splits * 2;
+    float m = -__builtin_inff();
+    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[2 * i]);
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    float l = 0.f, o[2] = {};
+    for (int i = 0; i < a.splits; ++i) {
+        const float w = __builtin_amdgcn_exp2f(ml[2 * i] - base);
+        l += w * ml[2 * i + 1];
+        const float *po = a.part_o + (row * a.splits + i) * DP;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (lane + j * 64 < a.D) o[j] += w * po[lane + j * 64];
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const long long bh = row / SG;
+    const int r = (int)(row - bh * SG), qi = r / a.G, g = r - qi * a.G;
+    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
+    T *out = (T *)a.out +
+             (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (lane + j * 64 < a.D) out[lane + j * 64] = (T)(o[j] * inv);
+    if (a.lse && lane == 0)
+        a.lse[row] = l == 0.f ? __builtin_inff() : base + log2f(l);
+}
+
+// ---- backward: dq, and delta = sum(dout * out) of each row ----
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_dq(const Args a)
+{
+    __shared__ Tile<DP> kt, vt;
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    const unsigned id = work_id();
+    const int bh = id / a.blocks;
+    const int blk = a.blocks - 1 - (int)(id - (unsigned)bh * a.blocks);
+    const int b = bh / a.Hk, h = bh - b * a.Hk;
+    const int SG = a.S * a.G;
+    const Seq s = sequence(a, b);
+    const int r0 = blk * 128, w0 = r0 + wid * 32;
+    const int rlast = r0 + 128 < SG ? r0 + 127 : SG - 1;
+    const int wlast = w0 + 31 < SG ? w0 + 31 : SG - 1;
+    const int r = w0 + lane % 32, qi = r / a.G, g = r - qi * a.G;
+    const int p = s.start + qi;
+    const View view = r < SG ? view_of(a, s, p) : View{0, -1, 0};
+    const bool live = r < SG && p >= 0 && p < s.n;
+    const int wp0 = s.start + w0 / a.G;
+    const int wp1 = w0 < SG ? s.start + wlast / a.G : INT_MIN / 2;
+    const int head = h * a.G + g;
+    const long long row = (long long)bh * SG + r;
+    const long long orow =
+        (((long long)b * a.S + qi) * a.Hk * a.G + head) * a.D;
+
+    s16x8 qop[DP / 16], gop[DP / 16];
+    float delta = 0.f;
+    {
+        const short *qrow = (const short *)a.q + b * a.qb + qi * a.qs +
+                            (long long)head * a.qh;
+        const short *grow = (const short *)a.dout + b * a.gb + qi * a.gs +
+                            (long long)head * a.gh;
+        const T *out = (const T *)a.o + orow;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int d = i * 16 + lane / 32 * 8;
+            s16x8 x = {}, y = {};
+            if (live && d < a.D) {
+                x = *(const s16x8 *)(qrow + d);
+                y = *(const s16x8 *)(grow + d);
+                float f[8];
+                ld8<T>(f, out + d);
+                const typename vec8<T>::type z =
+                    __builtin_bit_cast(typename vec8<T>::type, y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) delta += f[j] * (float)z[j];
+            }
+            qop[i] = x;
+            gop[i] = y;
+        }
+    }
+    delta += __shfl_xor(delta, 32);
+    const float lse = r < SG ? a.lse[row] : __builtin_inff();
+    if (r < SG && lane < 32) a.delta[row] = delta;
+
+    const Tiles tl =
+        tiles_of(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
+    const int end = tl.count();
+    const short *kbase = (const short *)a.k + b * a.kb + h * a.kh;
+    const short *vbase = (const short *)a.v + b * a.vb + h * a.vh;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
+
+    Stage<DP, 256> ks, vs;
+    if (end > 0) {
+        ks.load(kbase, a.ks, tl.at(0) * KT, s.n, a.D);
+        vs.load(vbase, a.vs, tl.at(0) * KT, s.n, a.D);
+    }
+    for (int i = 0; i < end; ++i) {
+        const int k0 = tl.at(i) * KT;
+        __syncthreads();
+        ks.store(kt);
+        vs.store(vt);
+        __syncthreads();
+        if (i + 1 < end) {
+            ks.load(kbase, a.ks, tl.at(i + 1) * KT, s.n, a.D);
+            vs.load(vbase, a.vs, tl.at(i + 1) * KT, s.n, a.D);
+        }
+        const int see = seen(a, s, wp0, wp1, k0, k0 + KT - 1);
+        if (see == 0) continue;
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+            f32x16 x = {}, y = {};
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                x = mfma<T>(rows_op<DP>(kt, t * 32, d, lane), qop[d], x);
+                y = mfma<T>(rows_op<DP>(vt, t * 32, d, lane), gop[d], y);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float w = __builtin_amdgcn_exp2f(x[e] * a.c - lse) *
+                          (y[e] - delta);
+                if (see == 1) {
+                    const int j = k0 + t * 32 + e / 4 * 8 + lane / 32 * 4 +
+                                  e % 4;
+                    if (!view.sees(j)) w = 0.f;
+                }
+                x[e] = w;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const s16x8 op = pack8<T>(x, u * 8);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+                    acc[d] = mfma<T>(
+                        cols_op<DP>(kt, t * 32 + u * 16, d, lane), op,
+                        acc[d]);
+            }
+        }
+    }
+    if (r >= SG) return;
+    T *out = (T *)a.dq + orow;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c0 = d * 32 + e * 8 + lane / 32 * 4;
+            typedef __attribute__((ext_vector_type(4))) T T4;
+            T4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = (T)(live ? acc[d][e * 4 + j] * a.scale : 0.f);
+            if (c0 < a.D) *(T4 *)(out + c0) = y;
+        }
+}
+
+// Rows that see any of keys k0..k1, as positions [p0, p1].
+__device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
+                               int &p0, int &p1)
+{
+    if (k1 > s.n - 1) k1 = s.n - 1;
+    const bool first = k0 < a.sinks;
+    p0 = a.causal ? k0 : first ? 0 : k0 - a.window + 1;
+    p1 = first || a.window > s.n - k1 ? s.n - 1 : k1 + a.window - 1;
+    if (k0 > k1) p1 = INT_MIN / 2;
+    if (p0 < 0) p0 = 0;
+    if (p0 < s.start) p0 = s.start;
+    if (p1 > s.n - 1) p1 = s.n - 1;
+    if (p1 > s.start + a.S - 1) p1 = s.start + a.S - 1;
+}
+
+// ---- backward: dk and dv ----
+// A wave owns 32 keys; tiles of rows of q and dout stream by. Key blocks
+// with first tokens are seen by all rows: they are split into parts of
+// `splits_rows` rows whose f32 sums attn_join_kv adds in order, and so are
+// the others where there are few blocks.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_dkv(const Args a)
+{
+    __shared__ Tile<DP> qt, gt;
+    __shared__ __align__(16) float lse_t[KT], delta_t[KT];
+    __shared__ __align__(16) int pos_t[KT];
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    const int units =
+        a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
+    const unsigned id = work_id();
+    const int bh = id / units;
+    int u = (int)(id - (unsigned)bh * units), blk, part, parts;
+    if (u < a.sink_blocks * a.sink_splits) {
+        parts = a.sink_splits;
+        blk = u / parts;
+        part = u - blk * parts;
+    } else {
+        u -= a.sink_blocks * a.sink_splits;
+        parts = a.splits;
+        blk = u / parts;
+        part = u - blk * parts;
+        blk += a.sink_blocks;
+    }
+    const int b = bh / a.Hk, h = bh - b * a.Hk;
+    const int SG = a.S * a.G;
+    const Seq s = sequence(a, b);
+    const int k0 = blk * 128, w0 = k0 + wid * 32;
+    const int key = w0 + lane % 32;
+
+    s16x8 kop[DP / 16], vop[DP / 16];
+    {
+        const short *krow = (const short *)a.k + b * a.kb +
+                            (long long)key * a.ks + h * a.kh;
+        const short *vrow = (const short *)a.v + b * a.vb +
+                            (long long)key * a.vs + h * a.vh;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int d = i * 16 + lane / 32 * 8;
+            s16x8 x = {}, y = {};
+            if (key < s.n && d < a.D) {
+                x = *(const s16x8 *)(krow + d);
+                y = *(const s16x8 *)(vrow + d);
+            }
+            kop[i] = x;
+            vop[i] = y;
+        }
+    }
+    int p0, p1;
+    rows_of(a, s, k0, k0 + 127, p0, p1);
+    int r0 = 0, r1 = 0;  // rows [r0, r1)
+    if (p0 <= p1) {
+        r0 = (p0 - s.start) * a.G;
+        r1 = (p1 - s.start + 1) * a.G;
+    }
+    if (parts > 1) {
+        const long long x = r0 + (long long)part * a.splits_rows;
+        const int stop = r1;
+        r0 = x < r1 ? (int)x : r1;
+        if (part < parts - 1 && r0 + (long long)a.splits_rows < stop)
+            r1 = r0 + a.splits_rows;
+    }
+
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = f32x16{};
+
+    // q and dout rows on their way; a row outside the sequence is zeros
+    constexpr int N = KT * DP / 8 / 256;
+    s16x8 qr[N], gr[N];
+    float lr = 0.f, dr = 0.f;
+    int pr = 0;
+    auto load = [&](int t0) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int slot = threadIdx.x + v * 256;
+            const int r = t0 + slot / (DP / 8), c = slot % (DP / 8) * 8;
+            s16x8 x = {}, y = {};
+            if (r < r1 && c < a.D) {
+                const int qi = r / a.G, head = h * a.G + r - qi * a.G;
+                x = *(const s16x8 *)((const short *)a.q + b * a.qb +
+                                     qi * a.qs + head * a.qh + c);
+                y = *(const s16x8 *)((const short *)a.dout + b * a.gb +
+                                     qi * a.gs + head * a.gh + c);
+            }
+            qr[v] = x;
+            gr[v] = y;
+        }
+        if (threadIdx.x < KT) {
+            const int r = t0 + threadIdx.x;
+            lr = __builtin_inff();
+            dr = 0.f;
+            pr = INT_MIN;
+            if (r < r1) {
+                lr = a.lse[(long long)bh * SG + r];
+                dr = a.delta[(long long)bh * SG + r];
+                pr = s.start + r / a.G;
+            }
+        }
+    };
+    if (r0 < r1) load(r0);
+    for (int t0 = r0; t0 < r1; t0 += KT) {
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int slot = threadIdx.x + v * 256;
+            const int at =
+                slot / (DP / 8) * Tile<DP>::LD + slot % (DP / 8) * 8;
+            *(s16x8 *)&qt.x[at] = qr[v];
+            *(s16x8 *)&gt.x[at] = gr[v];
+        }
+        if (threadIdx.x < KT) {
+            lse_t[threadIdx.x] = lr;
+            delta_t[threadIdx.x] = dr;
+            pos_t[threadIdx.x] = pr;
+        }
+        __syncthreads();
+        if (t0 + KT < r1) load(t0 + KT);
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+            const int f = t0 + t * 32;
+            if (f >= r1) break;
+            const int last = f + 31 < r1 ? f + 31 : r1 - 1;
+            const int see = seen(a, s, s.start + f / a.G,
+                                 s.start + last / a.G, w0, w0 + 31);
+            if (see == 0) continue;
+            f32x16 x = {}, y = {};
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                x = mfma<T>(rows_op<DP>(qt, t * 32, d, lane), kop[d], x);
+                y = mfma<T>(rows_op<DP>(gt, t * 32, d, lane), vop[d], y);
+            }
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const int at = t * 32 + e4 * 8 + lane / 32 * 4;
+                const f32x4 lse = *(const f32x4 *)&lse_t[at];
+                const f32x4 del = *(const f32x4 *)&delta_t[at];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = e4 * 4 + j;
+                    float w =
+                        __builtin_amdgcn_exp2f(x[e] * a.c - lse[j]);
+                    if (see == 1) {
+                        const View view = view_of(a, s, pos_t[at + j]);
+                        if (!view.sees(key)) w = 0.f;
+                    }
+                    x[e] = w;
+                    y[e] = w * (y[e] - del[j]);
+                    if (see == 1 && w == 0.f) y[e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const s16x8 pop = pack8<T>(x, v * 8);
+                const s16x8 sop = pack8<T>(y, v * 8);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    dv[d] = mfma<T>(
+                        cols_op<DP>(gt, t * 32 + v * 16, d, lane), pop,
+                        dv[d]);
+                    dk[d] = mfma<T>(
+                        cols_op<DP>(qt, t * 32 + v * 16, d, lane), sop,
+                        dk[d]);
+                }
+            }
+        }
+    }
+    if (key >= a.T) return;
+    if (parts > 1) {
+        // parts of a key head: sink blocks', then the others'
+        const long long slot =
+            blk < a.sink_blocks
+                ? (long long)blk * a.sink_splits + part
+                : (long long)a.sink_blocks * a.sink_splits +
+                      (long long)(blk - a.sink_blocks) * a.splits + part;
+        const long long at =
+            (((long long)bh * units + slot) * 128 + (key - k0)) * DP;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c0 = d * 32 + e * 8 + lane / 32 * 4;
+                f32x4 y, z;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = dk[d][e * 4 + j];
+                    z[j] = dv[d][e * 4 + j];
+                }
+                *(f32x4 *)(a.part_k + at + c0) = y;
+                *(f32x4 *)(a.part_v + at + c0) = z;
+            }
+        return;
+    }
+    const long long at =
+        (((long long)b * a.T + key) * a.Hk + h) * a.D;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c0 = d * 32 + e * 8 + lane / 32 * 4;
+            typedef __attribute__((ext_vector_type(4))) T T4;
+            T4 y, z;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                y[j] = (T)(dk[d][e * 4 + j] * a.scale);
+                z[j] = (T)dv[d][e * 4 + j];
+            }
+            if (c0 < a.D) {
+                *(T4 *)((T *)a.dk + at + c0) = y;
+                *(T4 *)((T *)a.dv + at + c0) = z;
+            }
+        }
+}
+
+// Adds the parts of dk and dv in order: one wave a key.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kv(const Args a, int DP)
+{
+    const int lane = threadIdx.x % WAVE;
+    const int blocks = a.splits > 1 ? a.blocks : a.sink_blocks;
+    const int units =
+        a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
+    const long long w = (long long)blockIdx.x * 4 + threadIdx.x / WAVE;
+    const long long bh = w / (blocks * 128);
+    if (bh >= (long long)a.B * a.Hk) return;
+    const int key = (int)(w - bh * blocks * 128);
+    if (key >= a.T) return;
+    const int blk = key / 128;
+    const bool sink = blk < a.sink_blocks;
+    const int parts = sink ? a.sink_splits : a.splits;
+    if (parts == 1) return;  // written where it was summed
+    const long long slot =
+        sink ? (long long)blk * a.sink_splits
+             : (long long)a.sink_blocks * a.sink_splits +
+                   (long long)(blk - a.sink_blocks) * a.splits;
+    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
+    const long long at = (((long long)b * a.T + key) * a.Hk + h) * a.D;
+    for (int c = lane; c < a.D; c += WAVE) {
+        float x = 0.f, y = 0.f;
+        for (int i = 0; i < parts; ++i) {
+            const long long from =
+                (((long long)bh * units + slot + i) * 128 + key % 128) * DP +
+                c;
+            x += a.part_k[from];
+            y += a.part_v[from];
+        }
+        ((T *)a.dk)[at + c] = (T)(x * a.scale);
+        ((T *)a.dv)[at + c] = (T)y;
+    }
+}
+
+// ---- how the work is cut ----
+constexpr int CUS = 256;
+
+inline int dp_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+// Most key tiles that a block of `rows` rows visits.
+long long most_tiles(const Args &a, int rows)
+{
+    long long keys = (rows + a.G - 1) / a.G;
+    if (a.window < a.T)
+        keys += (a.causal ? 1ll : 2ll) * a.window + a.sinks + 2 * KT;
+    else
+        keys = a.T;
+    if (keys > a.T) keys = a.T;
+    return (keys + KT - 1) / KT;
+}
+
+struct FwdPlan {
+    int waves, blocks, splits;
+};
+
+// Rows of a block: four waves of 32 share each key tile. Where that leaves
+// CUs without a block, blocks of one wave (when the rows fill no more),
+// and the keys are split until there are about four blocks a CU, with at
+// least four tiles each.
+FwdPlan plan_fwd(const Args &a)
+{
+    FwdPlan p;
+    const long long SG = (long long)a.S * a.G;
+    p.waves = SG <= 32 ? 1 : 4;
+    p.blocks = (int)((SG + p.waves * 32 - 1) / (p.waves * 32));
+    p.splits = 1;
+    const long long all = (long long)p.blocks * a.B * a.Hk;
+    const long long tiles = most_tiles(a, p.waves * 32);
+    const int want = p.waves == 1 ? 4 * CUS : CUS;
+    if (all < want) {
+        long long n = (want + all - 1) / all;
+        if (n > tiles / 4) n = tiles / 4;
+        if (n > 1) p.splits = (int)n;
+    }
+    return p;
+}
+
+// dk and dv: parts of at most as many rows as a block without first tokens
+// sees; shorter ones where the blocks are fewer than the CUs.
+void plan_dkv(Args &a)
+{
+    const long long SG = (long long)a.S * a.G;
+    a.blocks = (a.T + 127) / 128;
+    const long long sink =
+        a.window >= a.T ? 0
+                        : ((a.sinks < a.T ? a.sinks : a.T) + 127ll) / 128;
+    a.sink_blocks = (int)sink;
+    long long rows =
+        a.window >= a.T
+            ? SG
+            : (127ll + (a.causal ? 1ll : 2ll) * a.window) * a.G;
+    if (rows > SG) rows = SG;
+    long long piece = rows;
+    const long long bh = (long long)a.B * a.Hk;
+    const long long all = bh * a.blocks;
+    if (all < 2 * CUS) piece = rows * all / (2 * CUS);
+    if (piece < 256) piece = 256;
+    piece = (piece + KT - 1) / KT * KT;
+    a.splits_rows = (int)(piece < INT_MAX ? piece : INT_MAX);
+    a.splits = (int)((rows + piece - 1) / piece);
+    a.sink_splits = (int)((SG + piece - 1) / piece);
+    if (a.splits < 1) a.splits = 1;
+    if (a.sink_splits < 1) a.sink_splits = 1;
+}
+
+long long kv_units(const Args &a)
+{
+    return (long long)a.sink_blocks * a.sink_splits +
+           (long long)(a.blocks - a.sink_blocks) * a.splits;
+}
+
+bool kv_parts(const Args &a)
+{
+    return a.splits > 1 || (a.sink_blocks > 0 && a.sink_splits > 1);
+}
+
+template <typename T, int DP>
+hipError_t launch_fwd(Args &a, const FwdPlan &p, hipStream_t s)
+{
+    const long long n = (long long)a.B * a.Hk * p.blocks * p.splits;
+    if (n * 64 * p.waves >= 1ll << 32) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)n);
+    if (p.waves == 1) {
+        if (p.splits > 1)
+            attn_fwd<T, DP, 1, true><<<grid, 64, 0, s>>>(a);
+        else
+            attn_fwd<T, DP, 1, false><<<grid, 64, 0, s>>>(a);
+    } else {
+        if (p.splits > 1)
+            attn_fwd<T, DP, 4, true><<<grid, 256, 0, s>>>(a);
+        else
+            attn_fwd<T, DP, 4, false><<<grid, 256, 0, s>>>(a);
+    }
+    if (p.splits > 1) {
+        const long long rows = (long long)a.B * a.Hk * a.S * a.G;
+        attn_join<T><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a, DP);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, int DP>
+hipError_t launch_bwd(Args &a, hipStream_t s)
+{
+    const long long SG = (long long)a.S * a.G, bh = (long long)a.B * a.Hk;
+    Args d = a;
+    d.blocks = (int)((SG + 127) / 128);
+    const long long n = bh * d.blocks, m = bh * kv_units(a);
+    if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32)
+        return hipErrorInvalidValue;
+    if (n) attn_dq<T, DP><<<(unsigned)n, 256, 0, s>>>(d);
+    attn_dkv<T, DP><<<(unsigned)m, 256, 0, s>>>(a);
+    if (kv_parts(a)) {
+        const int blocks = a.splits > 1 ? a.blocks : a.sink_blocks;
+        attn_join_kv<T>
+            <<<(unsigned)(bh * blocks * 32), 256, 0, s>>>(a, DP);
+    }
+    return hipGetLastError();
+}
+
+// dims: B, S, T, Hk, G, D, window, sinks, causal
+void set_dims(Args &a, const long long *dims)
+{
+    a.B = (int)dims[0];
+    a.S = (int)dims[1];
+    a.T = (int)dims[2];
+    a.Hk = (int)dims[3];
+    a.G = (int)dims[4];
+    a.D = (int)dims[5];
+    a.window = (int)dims[6];
+    a.sinks = (int)dims[7];
+    a.causal = (int)dims[8];
+}
+
+// the limits that the kernels' 32-bit positions and rows rest on
+bool fits(const long long *d)
+{
+    for (int i = 0; i < 6; ++i)
+        if (d[i] < 1 || d[i] >= 1 << 30) return false;
+    return d[1] * d[4] < 1 << 30 && d[0] * d[3] < 1 << 30 && d[5] <= 128 &&
+           d[5] % 8 == 0 && d[6] >= 1 && d[6] <= 1 << 30 && d[7] >= 0 &&
+           d[7] <= 1 << 30;
+}
+
+}  // namespace
+
+extern "C" {
+
+// Workspace bytes of the forward (0 where the keys are not split) or the
+// backward; -1 where the sizes are out of range.
+long long kf_attn_ws(const long long *dims, int backward)
+{
+    if (!fits(dims)) return -1;
+    Args a = {};
+    set_dims(a, dims);
+    const long long rows = (long long)a.B * a.Hk * a.S * a.G;
+    const int DP = dp_of(a.D);
+    if (!backward) {
+        const FwdPlan p = plan_fwd(a);
+        return p.splits > 1 ? rows * p.splits * (DP + 2) * 4 : 0;
+    }
+    plan_dkv(a);
+    long long n = (rows * 4 + 255) / 256 * 256;  // delta
+    if (kv_parts(a))
+        n += 2ll * a.B * a.Hk * kv_units(a) * 128 * DP * 4;
+    return n;
+}
+
+// ptrs: q, k, v, out, lse (or 0), lengths, starts, workspace
+// strides: q (b s h), k, v in elements
+hipError_t kf_attn_fwd(const uintptr_t *ptrs, const long long *dims,
+                       const long long *st, float scale, int dtype,
+                       void *stream)
+{
+    if (!fits(dims)) return hipErrorInvalidValue;
+    Args a = {};
+    set_dims(a, dims);
+    a.q = (const void *)ptrs[0];
+    a.k = (const void *)ptrs[1];
+    a.v = (const void *)ptrs[2];
+    a.out = (void *)ptrs[3];
+    a.lse = (float *)ptrs[4];
+    a.lengths = (const int *)ptrs[5];
+    a.starts = (const int *)ptrs[6];
+    a.qb = st[0], a.qs = st[1], a.qh = st[2];
+    a.kb = st[3], a.ks = st[4], a.kh = st[5];
+    a.vb = st[6], a.vs = st[7], a.vh = st[8];
+    a.scale = scale;
+    a.c = scale * 1.44269504088896340736f;
+    const FwdPlan p = plan_fwd(a);
+    a.blocks = p.blocks;
+    a.splits = p.splits;
+    const int DP = dp_of(a.D);
+    a.part_o = (float *)ptrs[7];
+    a.part_ml =
+        a.part_o + (long long)a.B * a.Hk * a.S * a.G * p.splits * DP;
+    hipStream_t s = (hipStream_t)stream;
+#define CASE(N)                                                             \
+    if (DP == N)                                                            \
+    return dtype == 1   ? launch_fwd<__bf16, N>(a, p, s)                    \
+           : dtype == 2 ? launch_fwd<_Float16, N>(a, p, s)                  \
+                        : hipErrorInvalidValue
+    CASE(32);
+    CASE(64);
+    CASE(96);
+    CASE(128);
+#undef CASE
+    return hipErrorInvalidValue;
+}
+
+// ptrs: q, k, v, out, lse, lengths, starts, dout, dq, dk, dv, workspace
+// strides: q (b s h), k, v, dout in elements
+hipError_t kf_attn_bwd(const uintptr_t *ptrs, const long long *dims,
+                       const long long *st, float scale, int dtype,
+                       void *stream)
+{
+    if (!fits(dims)) return hipErrorInvalidValue;
+    Args a = {};
+    set_dims(a, dims);
+    a.q = (const void *)ptrs[0];
+    a.k = (const void *)ptrs[1];
+    a.v = (const void *)ptrs[2];
+    a.o = (const void *)ptrs[3];
+    a.lse = (float *)ptrs[4];
+    a.lengths = (const int *)ptrs[5];
+    a.starts = (const int *)ptrs[6];
+    a.dout = (const void *)ptrs[7];
+    a.dq = (void *)ptrs[8];
+    a.dk = (void *)ptrs[9];
+    a.dv = (void *)ptrs[10];
+    a.qb = st[0], a.qs = st[1], a.qh = st[2];
+    a.kb = st[3], a.ks = st[4], a.kh = st[5];
+    a.vb = st[6], a.vs = st[7], a.vh = st[8];
+    a.gb = st[9], a.gs = st[10], a.gh = st[11];
+    a.scale = scale;
+    a.c = scale * 1.44269504088896340736f;
+    plan_dkv(a);
+    const int DP = dp_of(a.D);
+    const long long rows = (long long)a.B * a.Hk * a.S * a.G;
+    a.delta = (float *)ptrs[11];
+    a.part_k = a.delta + (rows * 4 + 255) / 256 * 64;
+    a.part_v = a.part_k + (long long)a.B * a.Hk * kv_units(a) * 128 * DP;
+    hipStream_t s = (hipStream_t)stream;
+#define CASE(N)                                                             \
+    if (DP == N)                                                            \
+    return dtype == 1   ? launch_bwd<__bf16, N>(a, s)                       \
+           : dtype == 2 ? launch_bwd<_Float16, N>(a, s)                     \
+                        : hipErrorInvalidValue
+    CASE(32);
+    CASE(64);
+    CASE(96);
+    CASE(128);
+#undef CASE
+    return hipErrorInvalidValue;
+}
+
+}  // extern "C"

@@ -1,0 +1,133 @@
+"""Embedding lookup with a scale, and its gradient by sorted tokens.
+
+Wraps csrc/hip/embedding.hip. The lookup reads each row once and writes it
+scaled in the activations' type, with no cast pass after it. The gradient
+sums the rows of each token in one fixed order (a stable radix sort of the
+ids, no atomics), in f32 with one rounding at the end, so it repeats bit by
+bit; torch's nn.Embedding rounds after each of several steps and needs a
+cast of the gradient where the activations are of another type.
+
+On CPU tensors the same is computed by eager torch.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from kungfu_amd.ops import hip
+from kungfu_amd.utils.dtypes import hip_dtype
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check(ids, weight, padding_idx, out_dtype):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("ids must be int32 or int64, not %s" % ids.dtype)
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError("weight must be a (tokens, width) matrix, not %s" %
+                         (tuple(weight.shape),))
+    if ids.device != weight.device:
+        raise ValueError("ids are on %s, weight is on %s" %
+                         (ids.device, weight.device))
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError("padding_idx %d is outside %d tokens" %
+                         (padding_idx, weight.shape[0]))
+    if not weight.is_cuda:
+        return
+    if weight.dtype not in _FLOATS:
+        raise TypeError("weight must be float32, bfloat16 or float16, not "
+                        "%s" % weight.dtype)
+    if out_dtype not in (torch.float32, weight.dtype) and \
+            weight.dtype != torch.float32:
+        raise TypeError("no lookup of %s rows as %s" %
+                        (weight.dtype, out_dtype))
+    if out_dtype not in _FLOATS:
+        raise TypeError("no lookup as %s" % out_dtype)
+    if ids.numel() >= 1 << 30 or weight.shape[0] >= 1 << 30 or \
+            weight.shape[1] > 1 << 20:
+        raise ValueError("embedding is limited to 2^30 ids, 2^30 tokens and "
+                         "a width of 2^20")
+
+
+def _forward(ids, weight, scale, out_dtype):
+    h = hip._require()
+    w = weight if weight.stride(1) == 1 or weight.shape[1] == 1 else \
+        weight.contiguous()
+    out = torch.empty(ids.shape + weight.shape[1:], dtype=out_dtype,
+                      device=weight.device)
+    if ids.numel():
+        with hip.on_device(weight):
+            h.embed_fwd(ids.data_ptr(), ids.dtype == torch.int64,
+                        w.data_ptr(), w.stride(0), hip_dtype(w.dtype),
+                        out.data_ptr(), hip_dtype(out_dtype), ids.numel(),
+                        w.shape[0], w.shape[1], scale, hip.stream_of(w))
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.of = (weight.shape, weight.dtype, scale, padding_idx, out_dtype)
+        return _forward(ids, weight, scale, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        ids, = ctx.saved_tensors
+        (V, H), dtype, scale, padding_idx, out_dtype = ctx.of
+        h = hip._require()
+        dout = dout.to(out_dtype).contiguous()
+        dw = torch.empty((V, H), dtype=dtype, device=dout.device)
+        N = ids.numel()
+        with hip.on_device(dout):
+            ws = torch.empty(h.embed_ws(N, V, H), dtype=torch.uint8,
+                             device=dout.device)
+            h.embed_bwd(ids.data_ptr(), ids.dtype == torch.int64,
+                        dout.data_ptr(), hip_dtype(out_dtype), dw.data_ptr(),
+                        hip_dtype(dtype), N, V, H,
+                        -1 if padding_idx is None else padding_idx, scale,
+                        ws.data_ptr(), hip.stream_of(dout))
+        return None, dw, None, None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
+    """scale * weight[ids], as `out_dtype` (default: the weight's type).
+
+    ids: int32 or int64, any shape. weight: (tokens, width), f32, bf16 or
+    f16; `out_dtype` is f32 or the weight's type, or any of the three for
+    f32 weights. The row `padding_idx` is looked up as any other and gets no
+    gradient. The gradient is dense, of the weight's type.
+
+    An id outside the table raises on the CPU. On the GPU, where reading it
+    back would hold up the stream, its output row is NaN and it adds to no
+    gradient.
+    """
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    scale = float(scale)
+    _check(ids, weight, padding_idx, out_dtype)
+    if not weight.is_cuda:
+        rows = torch.nn.functional.embedding(ids, weight, padding_idx)
+        if weight.dtype != torch.float64:
+            rows = rows.float()
+        return (rows * scale).to(out_dtype)
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(ids, weight, scale, padding_idx, out_dtype)
+    return _forward(ids, weight, scale, out_dtype)
+
+
+class FusedEmbedding(torch.nn.Embedding):
+    """nn.Embedding with a scale and an output type of its own."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None,
+                 scale=1.0, out_dtype=None, **kwargs):
+        for name in ("max_norm", "scale_grad_by_freq", "sparse"):
+            if kwargs.get(name):
+                raise ValueError("FusedEmbedding has no %s" % name)
+        super().__init__(num_embeddings, embedding_dim, padding_idx,
+                         **kwargs)
+        self.scale = scale
+        self.out_dtype = out_dtype
+
+    def forward(self, ids):
+        return embedding(ids, self.weight, self.scale, self.padding_idx,
+                         self.out_dtype)

@@ -210,3 +210,44 @@ def transform2(z, x, op="sum"):
     _hip.transform2(z.data_ptr(), x.data_ptr(), z.numel(), ops[op],
                     hip_dtype(z.dtype), _stream())
     return z
+
+
+# ---- what the transformer ops share ----
+
+def on_device(t):
+    """Makes t's device current, for a launch on its stream."""
+    return torch.cuda.device(t.device)
+
+
+def stream_of(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def row_strides(t):
+    """Strides of the leading dimensions; 0 where the size is 1 (such a
+    stride is arbitrary and never used)."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+
+
+def rows16(t):
+    """t, or a copy of it, whose rows are dense and start at 16 bytes, as
+    the kernels that load 16 bytes at a time need."""
+    if t.numel() == 0:
+        return t
+    each = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+            all(s % each == 0 for s in row_strides(t)):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def check_ints(name, t, shapes, device):
+    """An int32 or int64 tensor of one of the shapes, on the device."""
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError("%s must be int32 or int64, not %s" % (name, t.dtype))
+    if tuple(t.shape) not in shapes:
+        raise ValueError("%s has shape %s, not %s" % (
+            name, tuple(t.shape), " or ".join(str(s) for s in shapes)))
+    if t.device != device:
+        raise ValueError("%s is on %s, not %s" % (name, t.device, device))

@@ -36,6 +36,9 @@ HIP_SOURCES = [
     "csrc/hip/kernels.hip",
     "csrc/hip/fused_bn.hip",
     "csrc/hip/fused_ln.hip",
+    "csrc/hip/embedding.hip",
+    "csrc/hip/qk_norm_rope.hip",
+    "csrc/hip/window_attention.hip",
     "csrc/hip/module_hip.cpp",
 ]
 
