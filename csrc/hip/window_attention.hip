@@ -243,7 +243,7 @@ __device__ inline unsigned work_id()
 // A wave owns 32 rows. SPLIT: the block takes one of `splits` parts of the
 // row block's tiles and writes the sums as they are, for attn_join.
 template <typename T, int DP, int NW, bool SPLIT>
-__global__ __launch_bounds__(NW *WAVE) void attn_fwd(const Args a)
+__global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
 {
     __shared__ Tile<DP> kt, vt;
     const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 
 // ---- backward: dq, and delta = sum(dout * out) of each row ----
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dq(const Args a)
+__global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
 {
     __shared__ Tile<DP> kt, vt;
     const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
@@ -599,7 +599,7 @@ __device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
 // `splits_rows` rows whose f32 sums attn_join_kv adds in order, and so are
 // the others where there are few blocks.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dkv(const Args a)
+__global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
 {
     __shared__ Tile<DP> qt, gt;
     __shared__ __align__(16) float lse_t[KT], delta_t[KT];
