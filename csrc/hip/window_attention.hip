@@ -53,7 +53,7 @@ struct Args {
     int splits;
     float *part_o, *part_ml;     // forward, split over keys
     float *part_k, *part_v;      // dk, dv, split over rows
-    int sink_blocks, sink_splits, splits_rows;
+    int sink_blocks, sink_splits, splits_rows, sink_rows;
 };
 
 template <typename T>
@@ -83,69 +83,104 @@ __device__ inline s16x8 pack8(const f32x16 &x, int at)
     return __builtin_bit_cast(s16x8, v);
 }
 
-// LDS tile: KT rows of DP elements, rows 16 bytes apart from a power of
-// two so that neighbouring rows start in other banks.
+// LDS tile: KT rows of DP elements in chunks of 16 bytes. Tiles are filled
+// by loads that go from memory to LDS without passing registers, which put
+// 64 lanes' chunks one after another: rows cannot be padded apart, so the
+// chunks of a row are permuted instead, c to c ^ f(row) within blocks of BS
+// chunks. f takes neighbouring rows' pairs of chunks (the transposing
+// read) and eight rows' single chunks (the plain one) to distinct banks.
 template <int DP>
 struct Tile {
-    static constexpr int LD = DP + 8;
-    __align__(16) short x[KT * LD];
+    static constexpr int CH = DP / 8;                      // chunks of a row
+    static constexpr int BS = DP == 128 ? 16 : DP == 64 ? 8 : 4;
+    __align__(1024) short x[KT * DP];
+
+    static __device__ inline int f(int row)
+    {
+        if (BS == 4) return (row >> 1 & 1) << 1 | (row >> 2 & 1);
+        return (row & 3) << 1 | (row >> 2 & 1) | (BS == 16 ? row & 8 : 0);
+    }
+    // byte of chunk `c` of `row`
+    static __device__ inline int at(int row, int c)
+    {
+        return row * DP * 2 + ((c & -BS) + ((c & (BS - 1)) ^ f(row))) * 16;
+    }
 };
 
 // A operand from rows r0..r0+31 as they lie: row r0 + l % 32, elements
-// 16 ks + 8 (l / 32) + 0..7.
+// 16 ks + 8 (l / 32) + 0..7. `at` is the lane's place for ks = 0, r0 = 0.
 template <int DP>
-__device__ inline s16x8 rows_op(const Tile<DP> &t, int r0, int ks, int lane)
+__device__ inline int rows_at(int lane)
 {
-    return *(const s16x8 *)&t.x[(r0 + lane % 32) * Tile<DP>::LD + ks * 16 +
-                                lane / 32 * 8];
+    return Tile<DP>::at(lane % 32, lane / 32);
+}
+template <int DP>
+__device__ inline s16x8 rows_op(const Tile<DP> &t, int at, int r0, int ks)
+{
+    constexpr int BS = Tile<DP>::BS;
+    const int c = ks * 2;
+    return *(const s16x8 *)((const char *)t.x +
+                            ((at ^ (c & (BS - 1)) << 4) + (c & -BS) * 16 +
+                             r0 * DP * 2));
 }
 
 // A operand of the transposed tile: row (of the operand) = element
 // 32 dt + l % 32, contracted index = tile rows r0 + 4 (l / 32) + 0..3 and
 // 8 rows on, the order in which the accumulators hold them.
 template <int DP>
-__device__ inline s16x8 cols_op(const Tile<DP> &t, int r0, int dt, int lane)
+__device__ inline int cols_at(int lane)
 {
     const int i = lane % 16;
-    const short *p = &t.x[(r0 + lane / 32 * 4 + i / 4) * Tile<DP>::LD +
-                          dt * 32 + lane / 16 % 2 * 16 + i % 4 * 4];
+    return Tile<DP>::at(lane / 32 * 4 + i / 4,
+                        lane / 16 % 2 * 2 + i % 4 / 2) +
+           i % 2 * 8;
+}
+template <int DP>
+__device__ inline s16x8 cols_op(const Tile<DP> &t, int at, int r0, int dt)
+{
+    constexpr int BS = Tile<DP>::BS;
+    const int c = dt * 4;
+    const char *p = (const char *)t.x + r0 * DP * 2 + (c & -BS) * 16;
     typedef __attribute__((address_space(3))) s16x4 lds4;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4 *)(p + (at ^ (c & (BS - 1)) << 4)));
+    // eight rows on; f has their bit where BS is 16
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds4 *)(p + 8 * Tile<DP>::LD));
+        (lds4 *)(p + 8 * DP * 2 +
+                 (at ^ ((c ^ (BS == 16 ? 8 : 0)) & (BS - 1)) << 4)));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A tile on its way from memory to LDS, NT threads.
-template <int DP, int NT>
-struct Stage {
-    static constexpr int N = KT * DP / 8 / NT;
-    s16x8 r[N];
-    // rows j0.. of a [T][D] matrix; rows outside [0, end) are zeros
-    __device__ void load(const void *base, long long stride, int j0, int end,
-                         int D)
-    {
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const int slot = threadIdx.x + v * NT;
-            const int row = slot / (DP / 8), c = slot % (DP / 8) * 8;
-            const int j = j0 + row;
-            s16x8 x = {};
-            if (j < end && c < D)
-                x = *(const s16x8 *)((const short *)base + j * stride + c);
-            r[v] = x;
-        }
+// Loads on their way into LDS are done, for this wave's part.
+__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Sends 16 bytes of each lane to 1 KiB of LDS from `to` (the same for all
+// lanes).
+__device__ inline void send16(const void *from, void *to)
+{
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void *)from,
+        (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// Sends rows j0.. of a matrix to a tile with NW waves. Rows past the last
+// one and columns past D repeat others, which hold nothing that could not
+// stand there: their scores are masked, their weights are zeros, and their
+// columns meet zeros or are not written.
+template <int DP, int NW, int U, typename Row>
+__device__ inline void send_tile(Tile<DP> &t, int wid, int lane, int D,
+                                 Row row_ptr)
+{
+    constexpr int CH = Tile<DP>::CH, BS = Tile<DP>::BS;
+#pragma unroll U
+    for (int v = 0; v < KT * CH / WAVE / NW; ++v) {
+        const int n0 = (v * NW + wid) * WAVE, n = n0 + lane;
+        const int row = n / CH, x = n % CH;
+        int c = (x & -BS) + ((x & (BS - 1)) ^ Tile<DP>::f(row));
+        if (c * 8 >= D) c = 0;
+        send16(row_ptr(row) + c * 8, (char *)t.x + n0 * 16);
     }
-    __device__ void store(Tile<DP> &t) const
-    {
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const int slot = threadIdx.x + v * NT;
-            const int row = slot / (DP / 8), c = slot % (DP / 8) * 8;
-            *(s16x8 *)&t.x[row * Tile<DP>::LD + c] = r[v];
-        }
-    }
-};
+}
 
 struct Seq {
     int n;      // keys
@@ -245,8 +280,9 @@ __device__ inline unsigned work_id()
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
 {
-    __shared__ Tile<DP> kt, vt;
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    __shared__ Tile<DP> kt0, kt1, vt0, vt1;
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     unsigned id = work_id();
     int split = 0;
     if (SPLIT) {
@@ -301,30 +337,35 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     float m = -__builtin_inff(), l = 0.f;
 
-    Stage<DP, NW * WAVE> ks, vs;
-    if (i < end) {
-        ks.load(kbase, a.ks, tl.at(i) * KT, s.n, a.D);
-        vs.load(vbase, a.vs, tl.at(i) * KT, s.n, a.D);
-    }
-    for (; i < end; ++i) {
+    const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
+        const int j0 = tile * KT;
+        auto krow = [&](int row) {
+            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
+            return kbase + j * a.ks;
+        };
+        auto vrow = [&](int row) {
+            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
+            return vbase + j * a.vs;
+        };
+        send_tile<DP, NW, 4>(kt, wid, lane, a.D, krow);
+        send_tile<DP, NW, 4>(vt, wid, lane, a.D, vrow);
+    };
+    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
+                    Tile<DP> &vn) {
         const int k0 = tl.at(i) * KT;
+        landed();
         __syncthreads();
-        ks.store(kt);
-        vs.store(vt);
-        __syncthreads();
-        if (i + 1 < end) {
-            ks.load(kbase, a.ks, tl.at(i + 1) * KT, s.n, a.D);
-            vs.load(vbase, a.vs, tl.at(i + 1) * KT, s.n, a.D);
-        }
+        if (i + 1 < end) send(tl.at(i + 1), kn, vn);
         const int see = seen(a, s, wp0, wp1, k0, k0 + KT - 1);
-        if (see == 0) continue;
+        if (see == 0) return;
         f32x16 x[KT / 32];
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             x[t] = f32x16{};
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d)
-                x[t] = mfma<T>(rows_op<DP>(kt, t * 32, d, lane), qop[d],
+                x[t] = mfma<T>(rows_op<DP>(kt, rat, t * 32, d), qop[d],
                                x[t]);
         }
         if (see == 1) {
@@ -366,8 +407,18 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
             const s16x8 pop = pack8<T>(x[t / 2], t % 2 * 8);
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
-                o[d] = mfma<T>(cols_op<DP>(vt, t * 16, d, lane), pop, o[d]);
+                o[d] = mfma<T>(cols_op<DP>(vt, cat, t * 16, d), pop,
+                               o[d]);
         }
+    };
+    if (i < end) send(tl.at(i), kt0, vt0);
+    // two buffers by name, so that reads of one are known not to touch
+    // what is on its way into the other
+    while (i < end) {
+        step(kt0, vt0, kt1, vt1);
+        if (++i >= end) break;
+        step(kt1, vt1, kt0, vt0);
+        ++i;
     }
     l += __shfl_xor(l, 32);
     if (r >= SG) return;
@@ -454,8 +505,9 @@ __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
 {
-    __shared__ Tile<DP> kt, vt;
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    __shared__ Tile<DP> kt0, kt1, vt0, vt1;
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const unsigned id = work_id();
     const int bh = id / a.blocks;
     const int blk = a.blocks - 1 - (int)(id - (unsigned)bh * a.blocks);
@@ -515,30 +567,36 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
 
-    Stage<DP, 256> ks, vs;
-    if (end > 0) {
-        ks.load(kbase, a.ks, tl.at(0) * KT, s.n, a.D);
-        vs.load(vbase, a.vs, tl.at(0) * KT, s.n, a.D);
-    }
-    for (int i = 0; i < end; ++i) {
+    const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
+        const int j0 = tile * KT;
+        auto krow = [&](int row) {
+            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
+            return kbase + j * a.ks;
+        };
+        auto vrow = [&](int row) {
+            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
+            return vbase + j * a.vs;
+        };
+        send_tile<DP, 4, 4>(kt, wid, lane, a.D, krow);
+        send_tile<DP, 4, 4>(vt, wid, lane, a.D, vrow);
+    };
+    int i = 0;
+    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
+                    Tile<DP> &vn) {
         const int k0 = tl.at(i) * KT;
+        landed();
         __syncthreads();
-        ks.store(kt);
-        vs.store(vt);
-        __syncthreads();
-        if (i + 1 < end) {
-            ks.load(kbase, a.ks, tl.at(i + 1) * KT, s.n, a.D);
-            vs.load(vbase, a.vs, tl.at(i + 1) * KT, s.n, a.D);
-        }
+        if (i + 1 < end) send(tl.at(i + 1), kn, vn);
         const int see = seen(a, s, wp0, wp1, k0, k0 + KT - 1);
-        if (see == 0) continue;
+        if (see == 0) return;
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             f32x16 x = {}, y = {};
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
-                x = mfma<T>(rows_op<DP>(kt, t * 32, d, lane), qop[d], x);
-                y = mfma<T>(rows_op<DP>(vt, t * 32, d, lane), gop[d], y);
+                x = mfma<T>(rows_op<DP>(kt, rat, t * 32, d), qop[d], x);
+                y = mfma<T>(rows_op<DP>(vt, rat, t * 32, d), gop[d], y);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -557,10 +615,19 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d)
                     acc[d] = mfma<T>(
-                        cols_op<DP>(kt, t * 32 + u * 16, d, lane), op,
+                        cols_op<DP>(kt, cat, t * 32 + u * 16, d), op,
                         acc[d]);
             }
         }
+    };
+    if (i < end) send(tl.at(i), kt0, vt0);
+    // two buffers by name, so that reads of one are known not to touch
+    // what is on its way into the other
+    while (i < end) {
+        step(kt0, vt0, kt1, vt1);
+        if (++i >= end) break;
+        step(kt1, vt1, kt0, vt0);
+        ++i;
     }
     if (r >= SG) return;
     T *out = (T *)a.dq + orow;
@@ -593,18 +660,25 @@ __device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
     if (p1 > s.start + a.S - 1) p1 = s.start + a.S - 1;
 }
 
+// What dk and dv need of a tile's rows.
+struct RowData {
+    __align__(16) float lse[KT];
+    __align__(16) float delta[KT];
+    __align__(16) int pos[KT];
+};
+
 // ---- backward: dk and dv ----
 // A wave owns 32 keys; tiles of rows of q and dout stream by. Key blocks
 // with first tokens are seen by all rows: they are split into parts of
 // `splits_rows` rows whose f32 sums attn_join_kv adds in order, and so are
 // the others where there are few blocks.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
+__global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
 {
-    __shared__ Tile<DP> qt, gt;
-    __shared__ __align__(16) float lse_t[KT], delta_t[KT];
-    __shared__ __align__(16) int pos_t[KT];
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    __shared__ Tile<DP> qt0, qt1, gt0, gt1;
+    __shared__ RowData rd0, rd1;
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
     const unsigned id = work_id();
@@ -653,68 +727,60 @@ __global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
         r1 = (p1 - s.start + 1) * a.G;
     }
     if (parts > 1) {
-        const long long x = r0 + (long long)part * a.splits_rows;
-        const int stop = r1;
+        const int piece = blk < a.sink_blocks ? a.sink_rows : a.splits_rows;
+        const long long x = r0 + (long long)part * piece;
         r0 = x < r1 ? (int)x : r1;
-        if (part < parts - 1 && r0 + (long long)a.splits_rows < stop)
-            r1 = r0 + a.splits_rows;
+        if (part < parts - 1 && r1 - r0 > piece) r1 = r0 + piece;
     }
+
+    // the rows that see this lane's key, as positions
+    int plo = 0, phi = -1;
+    if (key < s.n) rows_of(a, s, key, key, plo, phi);
 
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = f32x16{};
 
-    // q and dout rows on their way; a row outside the sequence is zeros
-    constexpr int N = KT * DP / 8 / 256;
-    s16x8 qr[N], gr[N];
-    float lr = 0.f, dr = 0.f;
-    int pr = 0;
-    auto load = [&](int t0) {
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const int slot = threadIdx.x + v * 256;
-            const int r = t0 + slot / (DP / 8), c = slot % (DP / 8) * 8;
-            s16x8 x = {}, y = {};
-            if (r < r1 && c < a.D) {
-                const int qi = r / a.G, head = h * a.G + r - qi * a.G;
-                x = *(const s16x8 *)((const short *)a.q + b * a.qb +
-                                     qi * a.qs + head * a.qh + c);
-                y = *(const s16x8 *)((const short *)a.dout + b * a.gb +
-                                     qi * a.gs + head * a.gh + c);
-            }
-            qr[v] = x;
-            gr[v] = y;
-        }
-        if (threadIdx.x < KT) {
-            const int r = t0 + threadIdx.x;
-            lr = __builtin_inff();
-            dr = 0.f;
-            pr = INT_MIN;
+    const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    // At 128 columns the operands and sums leave no registers for the
+    // addresses of several loads at once.
+    constexpr int U = DP > 96 ? 1 : 4;
+    // a row past the last one repeats it: its lse takes its weight to 0
+    auto send = [&](int t0, Tile<DP> &qt, Tile<DP> &gt, RowData &rd) {
+        auto qrow = [&](int row) {
+            const int r = t0 + row < r1 ? t0 + row : r1 - 1;
+            const int qi = r / a.G, head = h * a.G + r - qi * a.G;
+            return (const short *)a.q + b * a.qb + qi * a.qs + head * a.qh;
+        };
+        auto grow = [&](int row) {
+            const int r = t0 + row < r1 ? t0 + row : r1 - 1;
+            const int qi = r / a.G, head = h * a.G + r - qi * a.G;
+            return (const short *)a.dout + b * a.gb + qi * a.gs +
+                   head * a.gh;
+        };
+        send_tile<DP, 4, U>(qt, wid, lane, a.D, qrow);
+        send_tile<DP, 4, U>(gt, wid, lane, a.D, grow);
+        if (wid == 0) {
+            const int r = t0 + lane;
+            float l = __builtin_inff(), d = 0.f;
+            int p = INT_MIN;
             if (r < r1) {
-                lr = a.lse[(long long)bh * SG + r];
-                dr = a.delta[(long long)bh * SG + r];
-                pr = s.start + r / a.G;
+                l = a.lse[(long long)bh * SG + r];
+                d = a.delta[(long long)bh * SG + r];
+                p = s.start + r / a.G;
             }
+            rd.lse[lane] = l;
+            rd.delta[lane] = d;
+            rd.pos[lane] = p;
         }
     };
-    if (r0 < r1) load(r0);
-    for (int t0 = r0; t0 < r1; t0 += KT) {
+    int t0 = r0;
+    auto step = [&](const Tile<DP> &qt, const Tile<DP> &gt,
+                    const RowData &rd, Tile<DP> &qn, Tile<DP> &gn,
+                    RowData &rn) {
+        landed();
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const int slot = threadIdx.x + v * 256;
-            const int at =
-                slot / (DP / 8) * Tile<DP>::LD + slot % (DP / 8) * 8;
-            *(s16x8 *)&qt.x[at] = qr[v];
-            *(s16x8 *)&gt.x[at] = gr[v];
-        }
-        if (threadIdx.x < KT) {
-            lse_t[threadIdx.x] = lr;
-            delta_t[threadIdx.x] = dr;
-            pos_t[threadIdx.x] = pr;
-        }
-        __syncthreads();
-        if (t0 + KT < r1) load(t0 + KT);
+        if (t0 + KT < r1) send(t0 + KT, qn, gn, rn);
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             const int f = t0 + t * 32;
@@ -726,26 +792,33 @@ __global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
             f32x16 x = {}, y = {};
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
-                x = mfma<T>(rows_op<DP>(qt, t * 32, d, lane), kop[d], x);
-                y = mfma<T>(rows_op<DP>(gt, t * 32, d, lane), vop[d], y);
+                x = mfma<T>(rows_op<DP>(qt, rat, t * 32, d), kop[d], x);
+                y = mfma<T>(rows_op<DP>(gt, rat, t * 32, d), vop[d], y);
             }
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const int at = t * 32 + e4 * 8 + lane / 32 * 4;
-                const f32x4 lse = *(const f32x4 *)&lse_t[at];
-                const f32x4 del = *(const f32x4 *)&delta_t[at];
+                const f32x4 lse = *(const f32x4 *)&rd.lse[at];
+                const f32x4 del = *(const f32x4 *)&rd.delta[at];
+                float w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = __builtin_amdgcn_exp2f(x[e4 * 4 + j] * a.c -
+                                                  lse[j]);
+                if (see == 1) {
+                    const i32x4 pos = *(const i32x4 *)&rd.pos[at];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool on = pos[j] >= plo && pos[j] <= phi;
+                        w[j] = on ? w[j] : 0.f;
+                        // w = 0 times what a hidden row holds is 0 too
+                        y[e4 * 4 + j] = on ? y[e4 * 4 + j] : del[j];
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int e = e4 * 4 + j;
-                    float w =
-                        __builtin_amdgcn_exp2f(x[e] * a.c - lse[j]);
-                    if (see == 1) {
-                        const View view = view_of(a, s, pos_t[at + j]);
-                        if (!view.sees(key)) w = 0.f;
-                    }
-                    x[e] = w;
-                    y[e] = w * (y[e] - del[j]);
-                    if (see == 1 && w == 0.f) y[e] = 0.f;
+                    x[e4 * 4 + j] = w[j];
+                    y[e4 * 4 + j] = w[j] * (y[e4 * 4 + j] - del[j]);
                 }
             }
 #pragma unroll
@@ -755,14 +828,21 @@ __global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     dv[d] = mfma<T>(
-                        cols_op<DP>(gt, t * 32 + v * 16, d, lane), pop,
+                        cols_op<DP>(gt, cat, t * 32 + v * 16, d), pop,
                         dv[d]);
                     dk[d] = mfma<T>(
-                        cols_op<DP>(qt, t * 32 + v * 16, d, lane), sop,
+                        cols_op<DP>(qt, cat, t * 32 + v * 16, d), sop,
                         dk[d]);
                 }
             }
         }
+    };
+    if (t0 < r1) send(t0, qt0, gt0, rd0);
+    while (t0 < r1) {
+        step(qt0, gt0, rd0, qt1, gt1, rd1);
+        if ((t0 += KT) >= r1) break;
+        step(qt1, gt1, rd1, qt0, gt0, rd0);
+        t0 += KT;
     }
     if (key >= a.T) return;
     if (parts > 1) {
@@ -811,18 +891,18 @@ __global__ __launch_bounds__(256, DP > 96 ? 1 : 2) void attn_dkv(const Args a)
         }
 }
 
-// Adds the parts of dk and dv in order: one wave a key.
+// Adds the parts of dk and dv, one block a key: each wave a quarter of the
+// parts in order, then the quarters in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int DP)
 {
-    const int lane = threadIdx.x % WAVE;
+    __shared__ float part[4][2][128];
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
     const int blocks = a.splits > 1 ? a.blocks : a.sink_blocks;
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
-    const long long w = (long long)blockIdx.x * 4 + threadIdx.x / WAVE;
-    const long long bh = w / (blocks * 128);
-    if (bh >= (long long)a.B * a.Hk) return;
-    const int key = (int)(w - bh * blocks * 128);
+    const int bh = blockIdx.x / (blocks * 128);
+    const int key = blockIdx.x - bh * blocks * 128;
     if (key >= a.T) return;
     const int blk = key / 128;
     const bool sink = blk < a.sink_blocks;
@@ -832,20 +912,34 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int DP)
         sink ? (long long)blk * a.sink_splits
              : (long long)a.sink_blocks * a.sink_splits +
                    (long long)(blk - a.sink_blocks) * a.splits;
-    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
-    const long long at = (((long long)b * a.T + key) * a.Hk + h) * a.D;
-    for (int c = lane; c < a.D; c += WAVE) {
+    const long long from =
+        (((long long)bh * units + slot) * 128 + key % 128) * DP;
+    const int p0 = parts * wid / 4, p1 = parts * (wid + 1) / 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int c = lane + j * WAVE;
         float x = 0.f, y = 0.f;
-        for (int i = 0; i < parts; ++i) {
-            const long long from =
-                (((long long)bh * units + slot + i) * 128 + key % 128) * DP +
-                c;
-            x += a.part_k[from];
-            y += a.part_v[from];
+        if (c < a.D) {
+#pragma unroll 8
+            for (int i = p0; i < p1; ++i) {
+                x += a.part_k[from + (long long)i * 128 * DP + c];
+                y += a.part_v[from + (long long)i * 128 * DP + c];
+            }
         }
-        ((T *)a.dk)[at + c] = (T)(x * a.scale);
-        ((T *)a.dv)[at + c] = (T)y;
+        part[wid][0][c] = x;
+        part[wid][1][c] = y;
     }
+    __syncthreads();
+    const int c = threadIdx.x % 128, which = threadIdx.x / 128;
+    if (c >= a.D) return;
+    const float z = part[0][which][c] + part[1][which][c] +
+                    part[2][which][c] + part[3][which][c];
+    const int b = bh / a.Hk, h = bh - b * a.Hk;
+    const long long at = (((long long)b * a.T + key) * a.Hk + h) * a.D + c;
+    if (which)
+        ((T *)a.dv)[at] = (T)z;
+    else
+        ((T *)a.dk)[at] = (T)(z * a.scale);
 }
 
 // ---- how the work is cut ----
@@ -892,7 +986,11 @@ FwdPlan plan_fwd(const Args &a)
 }
 
 // dk and dv: parts of at most as many rows as a block without first tokens
-// sees; shorter ones where the blocks are fewer than the CUs.
+// sees, shorter ones where the blocks are fewer than the places for them.
+// The blocks with first tokens, which every row sees, are cut into eighths
+// of that, so that they fill up what the others leave at the end: 8192
+// tokens, 32/8 heads of 128, window 1024, has 504 blocks and 57 such
+// eighths a head for 512 places.
 void plan_dkv(Args &a)
 {
     const long long SG = (long long)a.S * a.G;
@@ -906,17 +1004,27 @@ void plan_dkv(Args &a)
             ? SG
             : (127ll + (a.causal ? 1ll : 2ll) * a.window) * a.G;
     if (rows > SG) rows = SG;
-    long long piece = rows;
     const long long bh = (long long)a.B * a.Hk;
     const long long all = bh * a.blocks;
-    if (all < 2 * CUS) piece = rows * all / (2 * CUS);
-    if (piece < 256) piece = 256;
-    piece = (piece + KT - 1) / KT * KT;
-    a.splits_rows = (int)(piece < INT_MAX ? piece : INT_MAX);
+    auto tiles = [](long long n) {  // at least 256 rows, whole tiles
+        n = n < 256 ? 256 : n;
+        return (n + KT - 1) / KT * KT;
+    };
+    const long long piece =
+        tiles(all < 2 * CUS ? rows * all / (2 * CUS) : rows);
+    a.splits_rows = (int)piece;
     a.splits = (int)((rows + piece - 1) / piece);
-    a.sink_splits = (int)((SG + piece - 1) / piece);
-    if (a.splits < 1) a.splits = 1;
-    if (a.sink_splits < 1) a.sink_splits = 1;
+    a.sink_rows = a.splits_rows;
+    a.sink_splits = 1;
+    if (sink) {
+        // their f32 sums take 1024 x 128 keys at most
+        const long long most = 4 * CUS / (bh * sink) + 1;
+        long long n = tiles(rows / 8);
+        if (n * most < SG) n = tiles(SG / most + 1);
+        if (n > piece) n = piece;
+        a.sink_rows = (int)n;
+        a.sink_splits = (int)((SG + n - 1) / n);
+    }
 }
 
 long long kv_units(const Args &a)
@@ -961,15 +1069,14 @@ hipError_t launch_bwd(Args &a, hipStream_t s)
     Args d = a;
     d.blocks = (int)((SG + 127) / 128);
     const long long n = bh * d.blocks, m = bh * kv_units(a);
-    if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32)
+    const bool parts = kv_parts(a);
+    const long long j =
+        parts ? bh * (a.splits > 1 ? a.blocks : a.sink_blocks) * 128 : 0;
+    if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32 || j * 256 >= 1ll << 32)
         return hipErrorInvalidValue;
     if (n) attn_dq<T, DP><<<(unsigned)n, 256, 0, s>>>(d);
     attn_dkv<T, DP><<<(unsigned)m, 256, 0, s>>>(a);
-    if (kv_parts(a)) {
-        const int blocks = a.splits > 1 ? a.blocks : a.sink_blocks;
-        attn_join_kv<T>
-            <<<(unsigned)(bh * blocks * 32), 256, 0, s>>>(a, DP);
-    }
+    if (parts) attn_join_kv<T><<<(unsigned)j, 256, 0, s>>>(a, DP);
     return hipGetLastError();
 }
 
