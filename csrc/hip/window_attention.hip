@@ -54,6 +54,7 @@ struct Args {
     float *part_o, *part_ml;     // forward, split over keys
     float *part_k, *part_v;      // dk, dv, split over rows
     int sink_blocks, sink_splits, splits_rows, sink_rows;
+    int even;  // G divides KT and a tile's offsets of rows fit 32 bits
 };
 
 template <typename T>
@@ -163,23 +164,100 @@ __device__ inline void send16(const void *from, void *to)
         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 }
 
-// Sends rows j0.. of a matrix to a tile with NW waves. Rows past the last
-// one and columns past D repeat others, which hold nothing that could not
-// stand there: their scores are masked, their weights are zeros, and their
-// columns meet zeros or are not written.
-template <int DP, int NW, int U, typename Row>
-__device__ inline void send_tile(Tile<DP> &t, int wid, int lane, int D,
-                                 Row row_ptr)
-{
-    constexpr int CH = Tile<DP>::CH, BS = Tile<DP>::BS;
-#pragma unroll U
-    for (int v = 0; v < KT * CH / WAVE / NW; ++v) {
-        const int n0 = (v * NW + wid) * WAVE, n = n0 + lane;
-        const int row = n / CH, x = n % CH;
-        int c = (x & -BS) + ((x & (BS - 1)) ^ Tile<DP>::f(row));
-        if (c * 8 >= D) c = 0;
-        send16(row_ptr(row) + c * 8, (char *)t.x + n0 * 16);
+// A lane's share of a tile that NW waves fill: which row and column its
+// v-th 16 bytes hold.
+template <int DP, int NW>
+struct Share {
+    static constexpr int CH = Tile<DP>::CH, BS = Tile<DP>::BS;
+    static constexpr int N = KT * CH / WAVE / NW;
+    static __device__ inline int row(int v, int wid, int lane)
+    {
+        return ((v * NW + wid) * WAVE + lane) / CH;
     }
+    static __device__ inline int col(int v, int wid, int lane, int D)
+    {
+        const int n = (v * NW + wid) * WAVE + lane, x = n % CH;
+        const int c = (x & -BS) + ((x & (BS - 1)) ^ Tile<DP>::f(n / CH));
+        return c * 8 < D ? c * 8 : 0;
+    }
+};
+
+// Sends rows of a matrix to a tile; at(v) is the address of the lane's v-th
+// piece. Rows past the last one and columns past D repeat others, which
+// hold nothing that could not stand there: their scores are masked, their
+// weights are zeros, and their columns meet zeros or are not written.
+template <int DP, int NW, int U, typename At>
+__device__ inline void send_tile(Tile<DP> &t, int wid, At at)
+{
+#pragma unroll U
+    for (int v = 0; v < Share<DP, NW>::N; ++v)
+        send16(at(v), (char *)t.x + (v * NW + wid) * WAVE * 16);
+}
+
+// Byte offsets of a lane's pieces of a tile from its first row. Where the
+// waves' loads take whole rows, the v-th piece lies `step` bytes (the same
+// for all lanes) after the one before.
+template <int DP, int NW>
+struct Offsets {
+    typedef Share<DP, NW> S;
+    static constexpr bool WHOLE = NW * WAVE % S::CH == 0 &&
+                                  NW * WAVE / S::CH % Tile<DP>::BS == 0;
+    static constexpr int ROWS = NW * WAVE / S::CH;  // of one v, if WHOLE
+    unsigned off[WHOLE ? 1 : S::N];
+    // row_off(row): elements of a row from the tile's first
+    template <typename F>
+    __device__ void set(int wid, int lane, int D, F row_off)
+    {
+#pragma unroll
+        for (int v = 0; v < (WHOLE ? 1 : S::N); ++v)
+            off[v] = 2u * (row_off(S::row(v, wid, lane)) +
+                           S::col(v, wid, lane, D));
+    }
+    // `step`: elements from a row to the one ROWS further
+    __device__ void send(Tile<DP> &t, const short *from, long long step,
+                         int wid) const
+    {
+        send_tile<DP, NW, 16>(t, wid, [&](int v) {
+            return WHOLE ? (const char *)(from + v * step) + off[0]
+                         : (const char *)from + off[WHOLE ? 0 : v];
+        });
+    }
+};
+
+// Keys and values: rows j0.. of a [T][D] matrix. Whole tiles take the
+// lane's offsets, which are the same for all of them, on a base that is
+// the same for all lanes; the last tile of a sequence stops at its end.
+template <int DP, int NW>
+struct KeyShare {
+    Offsets<DP, NW> o;
+    __device__ KeyShare(long long stride, int wid, int lane, int D)
+    {
+        o.set(wid, lane, D,
+              [&](int row) { return (unsigned)row * (unsigned)stride; });
+    }
+    __device__ void send(Tile<DP> &t, const short *base, long long stride,
+                         int j0, int end, int wid, int lane, int D) const
+    {
+        if (j0 + KT <= end) {
+            o.send(t, base + j0 * stride, Offsets<DP, NW>::ROWS * stride,
+                   wid);
+        } else {
+            send_tile<DP, NW, 1>(t, wid, [&](int v) {
+                int j = j0 + Share<DP, NW>::row(v, wid, lane);
+                j = j < end ? j : end - 1;
+                return base + j * stride +
+                       Share<DP, NW>::col(v, wid, lane, D);
+            });
+        }
+    }
+};
+
+// The value of the lane 32 lanes away.
+__device__ inline float other_half(float x)
+{
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
 }
 
 struct Seq {
@@ -266,13 +344,11 @@ __device__ inline int seen(const Args &a, const Seq &s, int p0, int p1,
     return 1;
 }
 
-// Neighbouring block ids run on different XCDs; give each XCD a
-// contiguous range of the work, so that blocks of one head share an L2.
-__device__ inline unsigned work_id()
-{
-    const unsigned n = gridDim.x / 8, id = blockIdx.x;
-    return id < n * 8 ? id % 8 * n + id / 8 : id;
-}
+// Work is handed out head by head for each block of rows or keys, the
+// blocks with most to do first: causal blocks that see much start before
+// those that see little, and blocks that share a CU are of all sizes.
+// Where the heads are a multiple of eight, a head stays on one XCD, since
+// neighbouring workgroups go to neighbouring XCDs.
 
 // ---- forward ----
 // A wave owns 32 rows. SPLIT: the block takes one of `splits` parts of the
@@ -283,15 +359,14 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     __shared__ Tile<DP> kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    unsigned id = work_id();
-    int split = 0;
+    const int heads = a.B * a.Hk;
+    int unit = blockIdx.x / heads, split = 0;
+    const int bh = blockIdx.x - unit * heads;
     if (SPLIT) {
-        split = id % a.splits;
-        id /= a.splits;
+        split = unit % a.splits;
+        unit /= a.splits;
     }
-    const int bh = id / a.blocks;
-    // later rows see more where causal: they go first
-    const int blk = a.blocks - 1 - (int)(id - (unsigned)bh * a.blocks);
+    const int blk = a.blocks - 1 - unit;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
@@ -338,18 +413,11 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     float m = -__builtin_inff(), l = 0.f;
 
     const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    const KeyShare<DP, NW> kshare(a.ks, wid, lane, a.D),
+        vshare(a.vs, wid, lane, a.D);
     auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
-        const int j0 = tile * KT;
-        auto krow = [&](int row) {
-            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
-            return kbase + j * a.ks;
-        };
-        auto vrow = [&](int row) {
-            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
-            return vbase + j * a.vs;
-        };
-        send_tile<DP, NW, 4>(kt, wid, lane, a.D, krow);
-        send_tile<DP, NW, 4>(vt, wid, lane, a.D, vrow);
+        kshare.send(kt, kbase, a.ks, tile * KT, s.n, wid, lane, a.D);
+        vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
     };
     auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
                     Tile<DP> &vn) {
@@ -383,12 +451,24 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top);
-        // a row that has seen nothing yet keeps zeros: exp2(-inf - 0)
-        const float base = mn == -__builtin_inff() ? 0.f : mn * a.c;
-        const float alpha = __builtin_amdgcn_exp2f(m * a.c - base);
-        m = mn;
+        top = fmaxf(top, other_half(top));
+        // m, which all weights are taken against, follows the maximum only
+        // when that is 2^8 over it: weights up to 2^8 keep the relative
+        // precision of the 16 bits they are rounded to, and the sums so
+        // far are seldom scaled
+        if (__any((top - m) * a.c > 8.f)) {
+            const float mn = fmaxf(m, top);
+            // a row that has seen nothing yet keeps zeros
+            const float alpha = __builtin_amdgcn_exp2f(
+                mn == -__builtin_inff() ? 0.f : (m - mn) * a.c);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        }
+        const float base = m == -__builtin_inff() ? 0.f : m * a.c;
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t)
@@ -397,11 +477,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
                 x[t][e] = __builtin_amdgcn_exp2f(x[t][e] * a.c - base);
                 sum += x[t][e];
             }
-        l = l * alpha + sum;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        l += sum;
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
             const s16x8 pop = pack8<T>(x[t / 2], t % 2 * 8);
@@ -420,7 +496,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         step(kt1, vt1, kt0, vt0);
         ++i;
     }
-    l += __shfl_xor(l, 32);
+    l += other_half(l);
     if (r >= SG) return;
     if (!live) {  // a tile that its neighbours see whole is not masked
         m = -__builtin_inff();
@@ -508,9 +584,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
     __shared__ Tile<DP> kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const unsigned id = work_id();
-    const int bh = id / a.blocks;
-    const int blk = a.blocks - 1 - (int)(id - (unsigned)bh * a.blocks);
+    const int heads = a.B * a.Hk, unit = blockIdx.x / heads;
+    const int bh = blockIdx.x - unit * heads, blk = a.blocks - 1 - unit;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
@@ -554,7 +629,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
             gop[i] = y;
         }
     }
-    delta += __shfl_xor(delta, 32);
+    delta += other_half(delta);
     const float lse = r < SG ? a.lse[row] : __builtin_inff();
     if (r < SG && lane < 32) a.delta[row] = delta;
 
@@ -568,18 +643,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
     for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
 
     const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    const KeyShare<DP, 4> kshare(a.ks, wid, lane, a.D),
+        vshare(a.vs, wid, lane, a.D);
     auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
-        const int j0 = tile * KT;
-        auto krow = [&](int row) {
-            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
-            return kbase + j * a.ks;
-        };
-        auto vrow = [&](int row) {
-            const int j = j0 + row < s.n ? j0 + row : s.n - 1;
-            return vbase + j * a.vs;
-        };
-        send_tile<DP, 4, 4>(kt, wid, lane, a.D, krow);
-        send_tile<DP, 4, 4>(vt, wid, lane, a.D, vrow);
+        kshare.send(kt, kbase, a.ks, tile * KT, s.n, wid, lane, a.D);
+        vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
     };
     int i = 0;
     auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
@@ -681,9 +749,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
-    const unsigned id = work_id();
-    const int bh = id / units;
-    int u = (int)(id - (unsigned)bh * units), blk, part, parts;
+    const int heads = a.B * a.Hk;
+    int u = blockIdx.x / heads, blk, part, parts;
+    const int bh = blockIdx.x - u * heads;
     if (u < a.sink_blocks * a.sink_splits) {
         parts = a.sink_splits;
         blk = u / parts;
@@ -741,25 +809,49 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = f32x16{};
 
-    const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
-    // At 128 columns the operands and sums leave no registers for the
-    // addresses of several loads at once.
-    constexpr int U = DP > 96 ? 1 : 4;
+    int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    // Where G divides the rows that the waves load at once, a lane's rows
+    // are the same queries and heads of every tile, at the same offsets
+    // from its first query.
+    typedef Offsets<DP, 4> Off;
+    const bool even = a.even && Off::ROWS % a.G == 0;
+    Off qo, go;
+    if (even) {
+        qo.set(wid, lane, a.D, [&](int row) {
+            const unsigned qi = row / a.G, g = row - qi * a.G;
+            return qi * (unsigned)a.qs + g * (unsigned)a.qh;
+        });
+        go.set(wid, lane, a.D, [&](int row) {
+            const unsigned qi = row / a.G, g = row - qi * a.G;
+            return qi * (unsigned)a.gs + g * (unsigned)a.gh;
+        });
+    }
+    const short *qbase =
+        (const short *)a.q + b * a.qb + (long long)h * a.G * a.qh;
+    const short *gbase =
+        (const short *)a.dout + b * a.gb + (long long)h * a.G * a.gh;
     // a row past the last one repeats it: its lse takes its weight to 0
     auto send = [&](int t0, Tile<DP> &qt, Tile<DP> &gt, RowData &rd) {
-        auto qrow = [&](int row) {
-            const int r = t0 + row < r1 ? t0 + row : r1 - 1;
-            const int qi = r / a.G, head = h * a.G + r - qi * a.G;
-            return (const short *)a.q + b * a.qb + qi * a.qs + head * a.qh;
-        };
-        auto grow = [&](int row) {
-            const int r = t0 + row < r1 ? t0 + row : r1 - 1;
-            const int qi = r / a.G, head = h * a.G + r - qi * a.G;
-            return (const short *)a.dout + b * a.gb + qi * a.gs +
-                   head * a.gh;
-        };
-        send_tile<DP, 4, U>(qt, wid, lane, a.D, qrow);
-        send_tile<DP, 4, U>(gt, wid, lane, a.D, grow);
+        if (even && t0 + KT <= r1) {
+            const int qi = t0 / a.G, step = Off::ROWS / a.G;
+            qo.send(qt, qbase + qi * a.qs, step * a.qs, wid);
+            go.send(gt, gbase + qi * a.gs, step * a.gs, wid);
+        } else {
+            auto row = [&](int v) {
+                const int r = t0 + Share<DP, 4>::row(v, wid, lane);
+                return r < r1 ? r : r1 - 1;
+            };
+            send_tile<DP, 4, 1>(qt, wid, [&](int v) {
+                const int r = row(v), qi = r / a.G, g = r - qi * a.G;
+                return qbase + qi * a.qs + g * a.qh +
+                       Share<DP, 4>::col(v, wid, lane, a.D);
+            });
+            send_tile<DP, 4, 1>(gt, wid, [&](int v) {
+                const int r = row(v), qi = r / a.G, g = r - qi * a.G;
+                return gbase + qi * a.gs + g * a.gh +
+                       Share<DP, 4>::col(v, wid, lane, a.D);
+            });
+        }
         if (wid == 0) {
             const int r = t0 + lane;
             float l = __builtin_inff(), d = 0.f;
@@ -789,12 +881,18 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
             const int see = seen(a, s, s.start + f / a.G,
                                  s.start + last / a.G, w0, w0 + 31);
             if (see == 0) continue;
+            // at 128 columns the sixteen places that follow from these two
+            // are not kept in registers over the loop
+            if (DP > 96) asm volatile("" : "+v"(rat), "+v"(cat));
             f32x16 x = {}, y = {};
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 x = mfma<T>(rows_op<DP>(qt, rat, t * 32, d), kop[d], x);
                 y = mfma<T>(rows_op<DP>(gt, rat, t * 32, d), vop[d], y);
             }
+            // the products' operands are not read ahead across the steps:
+            // there are no registers for them
+            if (DP > 96) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const int at = t * 32 + e4 * 8 + lane / 32 * 4;
@@ -821,6 +919,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
                     y[e4 * 4 + j] = w[j] * (y[e4 * 4 + j] - del[j]);
                 }
             }
+            if (DP > 96) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 const s16x8 pop = pack8<T>(x, v * 8);
@@ -1094,7 +1193,11 @@ void set_dims(Args &a, const long long *dims)
     a.causal = (int)dims[8];
 }
 
-// the limits that the kernels' 32-bit positions and rows rest on
+// elements whose bytes a 32-bit offset reaches
+bool near(long long n) { return n >= 0 && n < 1ll << 30; }
+
+// the limits that the kernels' 32-bit positions, rows and offsets in a tile
+// of keys rest on
 bool fits(const long long *d)
 {
     for (int i = 0; i < 6; ++i)
@@ -1147,6 +1250,7 @@ hipError_t kf_attn_fwd(const uintptr_t *ptrs, const long long *dims,
     a.qb = st[0], a.qs = st[1], a.qh = st[2];
     a.kb = st[3], a.ks = st[4], a.kh = st[5];
     a.vb = st[6], a.vs = st[7], a.vh = st[8];
+    if (!near(a.ks * KT) || !near(a.vs * KT)) return hipErrorInvalidValue;
     a.scale = scale;
     a.c = scale * 1.44269504088896340736f;
     const FwdPlan p = plan_fwd(a);
@@ -1193,10 +1297,13 @@ hipError_t kf_attn_bwd(const uintptr_t *ptrs, const long long *dims,
     a.qb = st[0], a.qs = st[1], a.qh = st[2];
     a.kb = st[3], a.ks = st[4], a.kh = st[5];
     a.vb = st[6], a.vs = st[7], a.vh = st[8];
+    if (!near(a.ks * KT) || !near(a.vs * KT)) return hipErrorInvalidValue;
     a.gb = st[9], a.gs = st[10], a.gh = st[11];
     a.scale = scale;
     a.c = scale * 1.44269504088896340736f;
     plan_dkv(a);
+    a.even = KT % a.G == 0 && near(a.qs * (KT / a.G) + a.qh * a.G) &&
+             near(a.gs * (KT / a.G) + a.gh * a.G);
     const int DP = dp_of(a.D);
     const long long rows = (long long)a.B * a.Hk * a.S * a.G;
     a.delta = (float *)ptrs[11];

@@ -231,12 +231,14 @@ def row_strides(t):
 
 def rows16(t):
     """t, or a copy of it, whose rows are dense and start at 16 bytes, as
-    the kernels that load 16 bytes at a time need."""
+    the kernels that load 16 bytes at a time need, and whose tokens
+    (dimension 1) are near enough for 32-bit offsets within a tile."""
     if t.numel() == 0:
         return t
     each = 16 // t.element_size()
+    strides = row_strides(t)
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % each == 0 for s in row_strides(t)):
+            all(s % each == 0 for s in strides) and strides[1] < 1 << 24:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
