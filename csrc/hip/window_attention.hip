@@ -360,13 +360,13 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int heads = a.B * a.Hk;
-    int unit = blockIdx.x / heads, split = 0;
-    const int bh = blockIdx.x - unit * heads;
+    int unit = blockIdx.x, split = 0;
     if (SPLIT) {
-        split = unit % a.splits;
         unit /= a.splits;
+        split = blockIdx.x - unit * a.splits;
     }
-    const int blk = a.blocks - 1 - unit;
+    const int blk = a.blocks - 1 - unit / heads;
+    const int bh = unit % heads;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
@@ -412,22 +412,16 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     float m = -__builtin_inff(), l = 0.f;
 
-    const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
+    int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
     const KeyShare<DP, NW> kshare(a.ks, wid, lane, a.D),
         vshare(a.vs, wid, lane, a.D);
-    auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
-        kshare.send(kt, kbase, a.ks, tile * KT, s.n, wid, lane, a.D);
-        vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
-    };
-    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
-                    Tile<DP> &vn) {
-        const int k0 = tl.at(i) * KT;
-        landed();
-        __syncthreads();
-        if (i + 1 < end) send(tl.at(i + 1), kn, vn);
-        const int see = seen(a, s, wp0, wp1, k0, k0 + KT - 1);
-        if (see == 0) return;
-        f32x16 x[KT / 32];
+    // Step u computes the scores of tile u and, in the same run of
+    // instructions, the weights and products of tile u - 1, so that the
+    // matrix pipe and the vector pipe both have work: 2 x 16 heads of 128,
+    // 8192 tokens, 891 TFLOP/s against 847 with one tile after another. It
+    // needs keys u and values u - 1 in LDS, and sends keys u + 1 and values
+    // u on their way.
+    auto score = [&](const Tile<DP> &kt, f32x16(&x)[KT / 32]) {
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             x[t] = f32x16{};
@@ -436,7 +430,28 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
                 x[t] = mfma<T>(rows_op<DP>(kt, rat, t * 32, d), qop[d],
                                x[t]);
         }
-        if (see == 1) {
+    };
+    auto weigh = [&](const Tile<DP> &vt, f32x16(&x)[KT / 32]) {
+        const float base = m == -__builtin_inff() ? 0.f : m * a.c;
+        float sum[4] = {};
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+#pragma unroll
+            for (int e = t % 2 * 8; e < t % 2 * 8 + 8; ++e) {
+                f32x16 &y = x[t / 2];
+                y[e] = __builtin_amdgcn_exp2f(y[e] * a.c - base);
+                sum[e % 4] += y[e];
+            }
+            const s16x8 pop = pack8<T>(x[t / 2], t % 2 * 8);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                o[d] = mfma<T>(cols_op<DP>(vt, cat, t * 16, d), pop, o[d]);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    // Hides what the mask hides of tile k0, and keeps m.
+    auto settle = [&](int k0, f32x16(&x)[KT / 32]) {
+        if (seen(a, s, wp0, wp1, k0, k0 + KT - 1) != 2) {
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
@@ -468,33 +483,51 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
         }
-        const float base = m == -__builtin_inff() ? 0.f : m * a.c;
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < KT / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                x[t][e] = __builtin_amdgcn_exp2f(x[t][e] * a.c - base);
-                sum += x[t][e];
-            }
-        l += sum;
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-            const s16x8 pop = pack8<T>(x[t / 2], t % 2 * 8);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
-                o[d] = mfma<T>(cols_op<DP>(vt, cat, t * 16, d), pop,
-                               o[d]);
-        }
     };
-    if (i < end) send(tl.at(i), kt0, vt0);
-    // two buffers by name, so that reads of one are known not to touch
-    // what is on its way into the other
-    while (i < end) {
-        step(kt0, vt0, kt1, vt1);
-        if (++i >= end) break;
-        step(kt1, vt1, kt0, vt0);
+    // A tile that this wave sees nothing of, of those that its block sees,
+    // is computed and masked as any other.
+    auto ready = [&](Tile<DP> &kn, Tile<DP> &vn) {
+        landed();
+        __syncthreads();
+        if (i + 1 < end)
+            kshare.send(kn, kbase, a.ks, tl.at(i + 1) * KT, s.n, wid, lane,
+                        a.D);
+        if (i < end)
+            vshare.send(vn, vbase, a.vs, tl.at(i) * KT, s.n, wid, lane, a.D);
+    };
+    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
+                    Tile<DP> &vn, f32x16(&xp)[KT / 32],
+                    f32x16(&x)[KT / 32]) {
+        ready(kn, vn);
+        // the places that follow from these two are worked out again: kept,
+        // they would take the registers of half a tile's scores
+        asm volatile("" : "+v"(rat), "+v"(cat));
+        score(kt, x);
+        weigh(vt, xp);
+        settle(tl.at(i) * KT, x);
         ++i;
+    };
+    if (i < end) {
+        f32x16 xa[KT / 32], xb[KT / 32];
+        kshare.send(kt0, kbase, a.ks, tl.at(i) * KT, s.n, wid, lane, a.D);
+        ready(kt1, vt0);
+        score(kt0, xa);
+        settle(tl.at(i) * KT, xa);
+        ++i;
+        // two buffers by name, so that reads of one are known not to touch
+        // what is on its way into the other
+        while (i + 1 < end) {
+            step(kt1, vt0, kt0, vt1, xa, xb);
+            step(kt0, vt1, kt1, vt0, xb, xa);
+        }
+        if (i < end) {
+            step(kt1, vt0, kt0, vt1, xa, xb);
+            ready(kt1, vt0);
+            weigh(vt1, xb);
+        } else {
+            ready(kt0, vt1);
+            weigh(vt0, xa);
+        }
     }
     l += other_half(l);
     if (r >= SG) return;
