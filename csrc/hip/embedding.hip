@@ -19,13 +19,17 @@ using namespace kfv;
 namespace {
 
 constexpr int BLOCK = 256;
-constexpr int SORT_TILE = 4096;           // keys a block ranks in one pass
-constexpr int SORT_ROUNDS = SORT_TILE / BLOCK;
 constexpr int WAVES = BLOCK / WAVE;
 constexpr int MAX_BITS = 8;               // digit bits of one pass
 constexpr int MAX_DIGITS = 1 << MAX_BITS;
+constexpr int SORT_TILE = 2048;           // keys a block ranks in one pass
+constexpr int SORT_ROUNDS = SORT_TILE / BLOCK;
+constexpr int SELF_SCAN = 64;  // blocks up to which each finds its own places
+constexpr int SMALL = 8192;    // keys up to which one block sorts them all
+constexpr int SMALL_BLOCK = 1024;
 constexpr int CHUNK = 32;                 // rows that one partial sum joins
 constexpr int COLS = WAVE * 8;            // columns that one wave sums
+constexpr int TWO_LEVELS = 16384;  // ids from which partial sums are joined
 
 __device__ inline unsigned load_key(const void *ids, int wide, long long n,
                                     long long V, long long padding)
@@ -38,46 +42,204 @@ __device__ inline unsigned load_key(const void *ids, int wide, long long n,
 // ---- forward ----
 // A block takes `rows` consecutive ids; its threads run over their vectors
 // of eight columns (VEC) or their columns one by one (rows that are not
-// 16-byte aligned), so that neighbours always touch neighbouring bytes.
+// 16-byte aligned), so that neighbours always touch neighbouring bytes, four
+// pieces at a time: the ids' loads go out together, and then the rows'.
 template <typename W, typename O, bool VEC>
 __global__ __launch_bounds__(BLOCK) void embed_fwd(
     const void *__restrict__ ids, int wide, const W *__restrict__ weight,
     long long ldw, O *__restrict__ out, long long N, long long V, int H,
     int rows, float scale)
 {
-    const int per = VEC ? H / 8 : H;
+    constexpr int U = 4, E = VEC ? 8 : 1;
+    const int per = H / E;
     for (long long n0 = (long long)blockIdx.x * rows; n0 < N;
          n0 += (long long)gridDim.x * rows) {
         const int here = (int)(N - n0 < rows ? N - n0 : rows);
-        for (int i = threadIdx.x; i < here * per; i += BLOCK) {
-            const int r = i / per, c = i - r * per;
-            const long long id = wide ? ((const long long *)ids)[n0 + r]
-                                      : (long long)((const int *)ids)[n0 + r];
-            const bool ok = id >= 0 && id < V;
-            if (VEC) {
-                float f[8];
-                if (ok) {
-                    ld8<W>(f, weight + id * ldw + c * 8);
+        const int all = here * per;
+        for (int i0 = threadIdx.x; i0 < all; i0 += U * BLOCK) {
+            int r[U], c[U];
+            bool ok[U];
+            long long id[U];
+            float f[U][E];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] *= scale;
-                } else {
+            for (int u = 0; u < U; ++u) {
+                int i = i0 + u * BLOCK;
+                i = i < all ? i : all - 1;
+                r[u] = i / per;
+                c[u] = (i - r[u] * per) * E;
+                id[u] = wide ? ((const long long *)ids)[n0 + r[u]]
+                             : (long long)((const int *)ids)[n0 + r[u]];
+            }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = __builtin_nanf("");
-                }
-                st8<O>(out + (n0 + r) * H + c * 8, f);
-            } else {
-                const float f = ok ? (float)weight[id * ldw + c] * scale
-                                   : __builtin_nanf("");
-                out[(n0 + r) * H + c] = (O)f;
+            for (int u = 0; u < U; ++u) {
+                ok[u] = id[u] >= 0 && id[u] < V;
+                const W *p = weight + (ok[u] ? id[u] : 0) * ldw + c[u];
+                if (VEC)
+                    ld8<W>(f[u], p);
+                else
+                    f[u][0] = (float)*p;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i0 + u * BLOCK >= all) break;
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    f[u][j] = ok[u] ? f[u][j] * scale : __builtin_nanf("");
+                O *to = out + (n0 + r[u]) * H + c[u];
+                if (VEC)
+                    st8<O>(to, f[u]);
+                else
+                    *to = (O)f[u][0];
             }
         }
     }
 }
 
 // ---- stable radix sort of (token, position), least digit first ----
-// One pass: hist counts the digits of each tile, scan turns the counts
-// (digit-major) into first places, scatter ranks the keys of a tile in
-// order and moves them. FIRST reads the ids themselves.
+
+// No token has rows until their bounds are found.
+__device__ inline void clear_spans(int *spans, long long V, long long at,
+                                   long long step)
+{
+    for (long long i = at; i < 2 * V; i += step) spans[i] = 0;
+}
+
+// Rank of each lane's digit among those of its wave that came before, in
+// the wave's own counters.
+__device__ inline unsigned wave_rank(unsigned d, bool in, int bits, int lane,
+                                     unsigned *cnt)
+{
+    unsigned long long same = __ballot(in);  // lanes with the same digit
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long one = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? one : ~one;
+    }
+    const unsigned before =
+        __builtin_popcountll(same & ((1ull << lane) - 1));
+    const unsigned rank = *(volatile unsigned *)&cnt[d] + before;
+    __builtin_amdgcn_wave_barrier();
+    if (in && before == 0)
+        *(volatile unsigned *)&cnt[d] = rank + __builtin_popcountll(same);
+    __builtin_amdgcn_wave_barrier();
+    return rank;
+}
+
+// Exclusive prefix sum over the N threads of a block, and the total.
+template <int N>
+__device__ inline unsigned block_scan(unsigned v, unsigned *wsum,
+                                      unsigned &total)
+{
+    const int lane = threadIdx.x % WAVE, w = threadIdx.x / WAVE;
+    unsigned inc = v;
+    for (int off = 1; off < WAVE; off <<= 1) {
+        const unsigned t = __shfl_up(inc, off);
+        if (lane >= off) inc += t;
+    }
+    if (lane == WAVE - 1) wsum[w] = inc;
+    __syncthreads();
+    unsigned before = 0;
+    total = 0;
+    for (int k = 0; k < N / WAVE; ++k) {
+        if (k < w) before += wsum[k];
+        total += wsum[k];
+    }
+    __syncthreads();
+    return before + inc - v;
+}
+
+// Few ids: block 0 sorts them all, keys and places in registers, one trip
+// through LDS for each digit; the other blocks clear the spans. 4096 ids of
+// 30522 tokens take 14 us, the passes below 35 us.
+__global__ __launch_bounds__(SMALL_BLOCK) void sort_small(
+    const void *__restrict__ ids, int wide, int N, long long V,
+    long long padding, int passes, int per, unsigned *__restrict__ keys,
+    unsigned *__restrict__ pos, int *__restrict__ spans)
+{
+    constexpr int ITEMS = SMALL / SMALL_BLOCK, NW = SMALL_BLOCK / WAVE;
+    __shared__ unsigned lkey[SMALL];
+    __shared__ unsigned short lpos[SMALL];
+    __shared__ unsigned cnt[NW][MAX_DIGITS];
+    __shared__ unsigned wsum[NW];
+    if (blockIdx.x) {
+        clear_spans(spans, V,
+                    (long long)(blockIdx.x - 1) * SMALL_BLOCK + threadIdx.x,
+                    (long long)(gridDim.x - 1) * SMALL_BLOCK);
+        return;
+    }
+    const int lane = threadIdx.x % WAVE, w = threadIdx.x / WAVE;
+    // a wave's keys lie together, so that wave order is key order; fewer
+    // keys are fewer rounds of every wave
+    const int rounds = (N + SMALL_BLOCK - 1) / SMALL_BLOCK;
+    const int base = w * rounds * WAVE + lane;
+    unsigned key[ITEMS], p[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const int n = base + r * WAVE;
+        key[r] = r < rounds && n < N ? load_key(ids, wide, n, V, padding)
+                                     : 0u;
+        p[r] = n;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * per;
+        const unsigned mask = (1u << per) - 1;
+        for (int i = threadIdx.x; i < NW * MAX_DIGITS; i += SMALL_BLOCK)
+            (&cnt[0][0])[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r)
+            if (r < rounds)
+                rank[r] = wave_rank((key[r] >> shift) & mask,
+                                    base + r * WAVE < N, per, lane, cnt[w]);
+        __syncthreads();
+        // places: digit by digit, and wave by wave within one
+        constexpr int EACH = MAX_DIGITS * NW / SMALL_BLOCK;
+        const int d = threadIdx.x * EACH / NW;
+        const int w0 = threadIdx.x * EACH % NW;
+        unsigned c[EACH], sum = 0, total;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            c[j] = cnt[w0 + j][d];
+            sum += c[j];
+        }
+        unsigned at = block_scan<SMALL_BLOCK>(sum, wsum, total);
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            cnt[w0 + j][d] = at;
+            at += c[j];
+        }
+        __syncthreads();
+        const bool last = pass == passes - 1;
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) {
+            if (r < rounds && base + r * WAVE < N) {
+                const unsigned to =
+                    cnt[w][(key[r] >> shift) & mask] + rank[r];
+                if (last) {
+                    keys[to] = key[r];
+                    pos[to] = p[r];
+                } else {
+                    lkey[to] = key[r];
+                    lpos[to] = (unsigned short)p[r];
+                }
+            }
+        }
+        if (last) break;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) {
+            const int n = base + r * WAVE;
+            if (r < rounds && n < N) {
+                key[r] = lkey[n];
+                p[r] = lpos[n];
+            }
+        }
+    }
+}
+
+// More ids: for each digit, hist counts the digits of each tile and scatter
+// ranks the keys of a tile in order and moves them; with many tiles, scan
+// turns the counts (digit-major) into first places in between. FIRST reads
+// the ids themselves; blocks past the last tile only clear the spans.
 template <bool FIRST>
 __global__ __launch_bounds__(BLOCK) void sort_hist(
     const void *__restrict__ src, int wide, long long N, long long V,
@@ -85,15 +247,16 @@ __global__ __launch_bounds__(BLOCK) void sort_hist(
     int nb, int *__restrict__ spans)
 {
     __shared__ unsigned cnt[MAX_DIGITS];
+    if (FIRST)
+        clear_spans(spans, V, (long long)blockIdx.x * BLOCK + threadIdx.x,
+                    (long long)gridDim.x * BLOCK);
+    if ((int)blockIdx.x >= nb) return;
     cnt[threadIdx.x] = 0;
     __syncthreads();
-    if (FIRST)  // no token has rows until bounds finds them
-        for (long long i = (long long)blockIdx.x * BLOCK + threadIdx.x;
-             i < 2 * V; i += (long long)gridDim.x * BLOCK)
-            spans[i] = 0;
-    const long long base = (long long)blockIdx.x * SORT_TILE;
+    const long long base = (long long)blockIdx.x * SORT_TILE + threadIdx.x;
+#pragma unroll
     for (int r = 0; r < SORT_ROUNDS; ++r) {
-        const long long n = base + r * BLOCK + threadIdx.x;
+        const long long n = base + r * BLOCK;
         if (n < N) {
             const unsigned key =
                 FIRST ? load_key(src, wide, n, V, padding)
@@ -111,40 +274,28 @@ __global__ __launch_bounds__(1024) void sort_scan(unsigned *__restrict__ hist,
                                                   int n)
 {
     __shared__ unsigned wsum[1024 / WAVE];
-    const int lane = threadIdx.x % WAVE, w = threadIdx.x / WAVE;
     unsigned carry = 0;
     for (int base = 0; base < n; base += 1024 * 4) {
         const int i0 = base + (int)threadIdx.x * 4;
-        unsigned v[4], s = 0;
+        unsigned v[4], s = 0, all;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             v[j] = i0 + j < n ? hist[i0 + j] : 0;
             s += v[j];
         }
-        unsigned inc = s;
-        for (int off = 1; off < WAVE; off <<= 1) {
-            const unsigned t = __shfl_up(inc, off);
-            if (lane >= off) inc += t;
-        }
-        if (lane == WAVE - 1) wsum[w] = inc;
-        __syncthreads();
-        unsigned before = carry, all = 0;
-        for (int k = 0; k < 1024 / WAVE; ++k) {
-            if (k < w) before += wsum[k];
-            all += wsum[k];
-        }
-        before += inc - s;
+        unsigned before = carry + block_scan<1024>(s, wsum, all);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (i0 + j < n) hist[i0 + j] = before;
             before += v[j];
         }
         carry += all;
-        __syncthreads();
     }
 }
 
-template <bool FIRST>
+// SCANNED: `place` holds first places; else counts, of at most SELF_SCAN
+// tiles, which every block sums for itself.
+template <bool FIRST, bool SCANNED>
 __global__ __launch_bounds__(BLOCK) void sort_scatter(
     const void *__restrict__ src, int wide,
     const unsigned *__restrict__ src_pos, long long N, long long V,
@@ -154,10 +305,10 @@ __global__ __launch_bounds__(BLOCK) void sort_scatter(
 {
     // keys of one wave lie together, so wave order is key order
     __shared__ unsigned cnt[WAVES][MAX_DIGITS];
+    __shared__ unsigned wsum[WAVES];
     const int lane = threadIdx.x % WAVE, w = threadIdx.x / WAVE;
     for (int i = threadIdx.x; i < WAVES * MAX_DIGITS; i += BLOCK)
         (&cnt[0][0])[i] = 0;
-    __syncthreads();
     const long long base = (long long)blockIdx.x * SORT_TILE +
                            w * (SORT_TILE / WAVES) + lane;
     unsigned key[SORT_ROUNDS], rank[SORT_ROUNDS];
@@ -168,29 +319,29 @@ __global__ __launch_bounds__(BLOCK) void sort_scatter(
                  : FIRST ? load_key(src, wide, n, V, padding)
                          : ((const unsigned *)src)[n];
     }
-#pragma unroll
-    for (int r = 0; r < SORT_ROUNDS; ++r) {
-        const bool in = base + r * WAVE < N;
-        const unsigned d = (key[r] >> shift) & ((1u << bits) - 1);
-        // lanes with the same digit
-        unsigned long long same = __ballot(in);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long one = __ballot((d >> b) & 1);
-            same &= (d >> b) & 1 ? one : ~one;
+    const int d = threadIdx.x;
+    unsigned at = 0;
+    if (SCANNED) {
+        if (d < 1 << bits) at = place[(long long)d * nb + blockIdx.x];
+    } else {
+        unsigned mine = 0, all = 0, total;
+        if (d < 1 << bits) {
+#pragma unroll 8
+            for (int i = 0; i < nb; ++i) {
+                const unsigned c = place[d * nb + i];
+                if (i < (int)blockIdx.x) mine += c;
+                all += c;
+            }
         }
-        const unsigned before = __builtin_popcountll(
-            same & ((1ull << lane) - 1));
-        rank[r] = *(volatile unsigned *)&cnt[w][d] + before;
-        __builtin_amdgcn_wave_barrier();
-        if (in && before == 0)
-            *(volatile unsigned *)&cnt[w][d] =
-                rank[r] + __builtin_popcountll(same);
-        __builtin_amdgcn_wave_barrier();
+        at = block_scan<BLOCK>(all, wsum, total) + mine;
     }
     __syncthreads();
-    const int d = threadIdx.x;
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r)
+        rank[r] = wave_rank((key[r] >> shift) & ((1u << bits) - 1),
+                            base + r * WAVE < N, bits, lane, cnt[w]);
+    __syncthreads();
     if (d < 1 << bits) {
-        unsigned at = place[(long long)d * nb + blockIdx.x];
         for (int k = 0; k < WAVES; ++k) {
             const unsigned c = cnt[k][d];
             cnt[k][d] = at;
@@ -210,89 +361,121 @@ __global__ __launch_bounds__(BLOCK) void sort_scatter(
     }
 }
 
-// spans[v] = {first, one past the last} place of token v
-__global__ __launch_bounds__(BLOCK) void token_bounds(
-    const unsigned *__restrict__ keys, long long N, unsigned V,
-    int *__restrict__ spans)
+// ---- sums of the rows of each token ----
+// A wave sums 512 columns, eight a lane, in groups of `PER` neighbours: as
+// many as 16 bytes of dW hold (VEC), or one by one.
+template <typename W, bool VEC>
+struct Cols {
+    static constexpr int PER = VEC ? 16 / (int)sizeof(W) : 1;
+    static constexpr int GROUPS = 8 / PER;
+    // first column of the lane's group g
+    static __device__ inline int at(int c0, int lane, int g)
+    {
+        return c0 + (g * WAVE + lane) * PER;
+    }
+};
+
+template <typename T, int PER>
+__device__ inline void load_n(float *f, const T *p)
 {
-    const long long n = (long long)blockIdx.x * BLOCK + threadIdx.x;
-    if (n >= N) return;
-    const unsigned k = keys[n];
-    if (k >= V) return;
-    if (n == 0 || keys[n - 1] != k) spans[2 * (long long)k] = (int)n;
-    if (n == N - 1 || keys[n + 1] != k) spans[2 * (long long)k + 1] = (int)n + 1;
+    constexpr int A = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
+    typedef __attribute__((ext_vector_type(PER), aligned(A))) T V;
+    const V v = *(const V *)p;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) f[i] = (float)v[i];
+}
+template <typename T, int PER>
+__device__ inline void store_n(T *p, const float *f)
+{
+    constexpr int A = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
+    typedef __attribute__((ext_vector_type(PER), aligned(A))) T V;
+    V v;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = (T)f[i];
+    *(V *)p = v;
 }
 
-// Columns of lane `lane`: eight neighbours (VEC), or every 64th.
-template <bool VEC>
-__device__ inline int col_of(int c0, int lane, int j)
+// acc += rows of `base`, `n` of them at most U, that idx(i) numbers: all
+// loads go out before the first sum.
+template <typename T, typename C, int U, typename Idx>
+__device__ inline void add_rows(float *acc, const T *base, int n, int c0,
+                                int lane, int H, Idx idx)
 {
-    return VEC ? c0 + lane * 8 + j : c0 + j * WAVE + lane;
-}
-
-template <typename T, bool VEC>
-__device__ inline void add_row(float *acc, const T *row, int c0, int lane,
-                               int H)
-{
-    if (VEC) {
-        if (c0 + lane * 8 < H) {
-            float f[8];
-            ld8<T>(f, row + c0 + lane * 8);
+    float f[U][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += f[j];
-        }
-    } else {
+    for (int u = 0; u < U; ++u) {
+        const T *row = base + (long long)idx(u < n ? u : 0) * H;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = col_of<VEC>(c0, lane, j);
-            if (c < H) acc[j] += (float)row[c];
+        for (int g = 0; g < C::GROUPS; ++g) {
+            // a branch around a load would wait for it; lanes past the
+            // last column repeat it, and their sums are not stored
+            const int c = C::at(c0, lane, g);
+            load_n<T, C::PER>(&f[u][g * C::PER],
+                              row + (c < H ? c : H - C::PER));
         }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += f[u][j];
 }
 
 // Sums of CHUNK neighbours of the sorted order that belong to one token,
 // so that a frequent token's row is not one long chain of reads. Level 1
-// sums rows of dout, level 2 sums level 1's results.
-template <typename T, bool VEC, int LEVEL>
+// sums rows of dout and finds where each token's places begin and end;
+// level 2 sums level 1's results.
+template <typename T, typename W, bool VEC, int LEVEL>
 __global__ __launch_bounds__(BLOCK) void embed_partial(
     const unsigned *__restrict__ keys, const unsigned *__restrict__ pos,
     const T *__restrict__ dout, const float *__restrict__ part1,
-    float *__restrict__ part, long long N, unsigned V, int H, int slices)
+    float *__restrict__ part, int *__restrict__ spans, long long N,
+    unsigned V, int H, int slices)
 {
-    const int lane = threadIdx.x % WAVE;
-    const long long unit = __builtin_amdgcn_readfirstlane(
-        (int)(blockIdx.x * WAVES + threadIdx.x / WAVE));
-    const long long chunk = unit / slices;
-    const int c0 = (int)(unit - chunk * slices) * COLS;
+    typedef Cols<W, VEC> C;
     constexpr int SPAN = LEVEL == 1 ? CHUNK : CHUNK * CHUNK;
-    const long long i0 = chunk * SPAN;
+    const int lane = threadIdx.x % WAVE;
+    const int unit = __builtin_amdgcn_readfirstlane(
+        (int)(blockIdx.x * WAVES + threadIdx.x / WAVE));
+    const int chunk = unit / slices, slice = unit - chunk * slices;
+    const long long i0 = (long long)chunk * SPAN;
+    if (i0 >= N) return;
+    if (LEVEL == 1 && slice == 0 && lane < CHUNK && i0 + lane < N) {
+        const long long n = i0 + lane;
+        const unsigned k = keys[n];
+        if (k < V) {
+            if (n == 0 || keys[n - 1] != k)
+                spans[2 * (long long)k] = (int)n;
+            if (n == N - 1 || keys[n + 1] != k)
+                spans[2 * (long long)k + 1] = (int)n + 1;
+        }
+    }
     if (i0 + SPAN > N) return;
     const unsigned k = keys[i0];
     if (k >= V || keys[i0 + SPAN - 1] != k) return;
+    const int c0 = slice * COLS;
     float acc[8] = {};
-#pragma unroll 8
-    for (int i = 0; i < CHUNK; ++i) {
+#pragma unroll 1
+    for (int i = 0; i < CHUNK; i += 16) {
         if (LEVEL == 1)
-            add_row<T, VEC>(acc, dout + (long long)pos[i0 + i] * H, c0,
-                            lane, H);
+            add_rows<T, C, 16>(acc, dout, 16, c0, lane, H,
+                               [&](int u) { return pos[i0 + i + u]; });
         else
-            add_row<float, VEC>(acc, part1 + (chunk * CHUNK + i) * H, c0,
-                                lane, H);
+            add_rows<float, C, 16>(acc, part1, 16, c0, lane, H, [&](int u) {
+                return chunk * CHUNK + i + u;
+            });
     }
-    float *row = part + chunk * H;
-    if (VEC) {
-        if (c0 + lane * 8 < H) st8<float>(row + c0 + lane * 8, acc);
-    } else {
+    float *row = part + (long long)chunk * H;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = col_of<VEC>(c0, lane, j);
-            if (c < H) row[c] = acc[j];
-        }
+    for (int g = 0; g < C::GROUPS; ++g) {
+        const int c = C::at(c0, lane, g);
+        if (c < H) store_n<float, C::PER>(row + c, &acc[g * C::PER]);
     }
 }
 
 // One wave writes 512 columns of one row of dW: zeros, or the token's rows
-// in their order, whole chunks by their partial sums.
+// in their order, whole chunks (and chunks of chunks, where part2 holds
+// them) by their partial sums.
 template <typename T, typename W, bool VEC>
 __global__ __launch_bounds__(BLOCK) void embed_rows(
     const int *__restrict__ spans, const unsigned *__restrict__ pos,
@@ -300,6 +483,7 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
     const float *__restrict__ part2, W *__restrict__ dw, long long units,
     int H, int slices, float scale)
 {
+    typedef Cols<W, VEC> C;
     const int lane = threadIdx.x % WAVE;
     for (long long u = (long long)blockIdx.x * WAVES + threadIdx.x / WAVE;
          u < units; u += (long long)gridDim.x * WAVES) {
@@ -310,35 +494,45 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
         const int end = spans[2 * (long long)v + 1];
         float acc[8] = {};
         while (i < end) {
-            if (i % CHUNK == 0 && end - i >= CHUNK) {
-                constexpr int BIG = CHUNK * CHUNK;
-                if (i % BIG == 0 && end - i >= BIG) {
-                    add_row<float, VEC>(acc, part2 + (long long)(i / BIG) * H,
-                                        c0, lane, H);
-                    i += BIG;
-                } else {
-                    add_row<float, VEC>(acc,
-                                        part1 + (long long)(i / CHUNK) * H,
-                                        c0, lane, H);
-                    i += CHUNK;
-                }
+            constexpr int BIG = CHUNK * CHUNK;
+            const int left = end - i;
+            if (i % CHUNK || left < CHUNK) {
+                // up to the next chunk, or to the end
+                const int here = CHUNK - i % CHUNK;
+                int n = here < left ? here : left;
+                n = n < 8 ? n : 8;
+                if (n == 1)
+                    add_rows<T, C, 1>(acc, dout, 1, c0, lane, H,
+                                      [&](int) { return pos[i]; });
+                else
+                    add_rows<T, C, 8>(acc, dout, n, c0, lane, H,
+                                      [&](int k) { return pos[i + k]; });
+                i += n;
+            } else if (!part2 || i % BIG || left < BIG) {
+                // up to the next chunk of chunks, or to the last chunk
+                int n = left / CHUNK;
+                const int here = (BIG - i % BIG) / CHUNK;
+                n = part2 && here < n ? here : n;
+                n = n < 8 ? n : 8;
+                add_rows<float, C, 8>(acc, part1, n, c0, lane, H, [&](int k) {
+                    return i / CHUNK + k;
+                });
+                i += n * CHUNK;
             } else {
-                add_row<T, VEC>(acc, dout + (long long)pos[i] * H, c0, lane,
-                                H);
-                i += 1;
+                int n = left / BIG;
+                n = n < 8 ? n : 8;
+                add_rows<float, C, 8>(acc, part2, n, c0, lane, H,
+                                      [&](int k) { return i / BIG + k; });
+                i += n * BIG;
             }
         }
+        W *row = dw + (long long)v * H;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] *= scale;
-        W *row = dw + (long long)v * H;
-        if (VEC) {
-            if (c0 + lane * 8 < H) st8<W>(row + c0 + lane * 8, acc);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = col_of<VEC>(c0, lane, j);
-                if (c < H) row[c] = (W)acc[j];
-            }
+        for (int g = 0; g < C::GROUPS; ++g) {
+            const int c = C::at(c0, lane, g);
+            if (c < H) store_n<W, C::PER>(row + c, &acc[g * C::PER]);
         }
     }
 }
@@ -352,7 +546,7 @@ struct Workspace {
     size_t bytes;
     Workspace(char *p, long long N, long long V, int H)
     {
-        const long long nb = N / SORT_TILE + 1;
+        const long long nb = (N + SORT_TILE - 1) / SORT_TILE;
         size_t at = 0;
         auto take = [&](size_t n) {
             char *q = p + at;
@@ -399,23 +593,26 @@ hipError_t sums(const Workspace &ws, int at, const void *dout, void *dw,
                 long long N, long long V, int H, float scale, hipStream_t s)
 {
     const int slices = (H + COLS - 1) / COLS;
-    const long long n1 = N / CHUNK * slices;
+    const long long n1 = (N + CHUNK - 1) / CHUNK * slices;
     if (n1)
-        embed_partial<T, VEC, 1>
+        embed_partial<T, W, VEC, 1>
             <<<(unsigned)((n1 + WAVES - 1) / WAVES), BLOCK, 0, s>>>(
                 ws.keys[at], ws.pos[at], (const T *)dout, nullptr, ws.part1,
-                N, (unsigned)V, H, slices);
-    const long long n2 = N / (CHUNK * CHUNK) * slices;
-    if (n2)
-        embed_partial<T, VEC, 2>
+                ws.spans, N, (unsigned)V, H, slices);
+    const float *part2 = nullptr;
+    if (N >= TWO_LEVELS) {
+        part2 = ws.part2;
+        const long long n2 = N / (CHUNK * CHUNK) * slices;
+        embed_partial<T, W, VEC, 2>
             <<<(unsigned)((n2 + WAVES - 1) / WAVES), BLOCK, 0, s>>>(
-                ws.keys[at], ws.pos[at], nullptr, ws.part1, ws.part2, N,
-                (unsigned)V, H, slices);
+                ws.keys[at], ws.pos[at], nullptr, ws.part1, ws.part2,
+                nullptr, N, (unsigned)V, H, slices);
+    }
     const long long units = V * slices;
     long long blocks = (units + WAVES - 1) / WAVES;
     if (blocks > 1 << 20) blocks = 1 << 20;
     embed_rows<T, W, VEC><<<(unsigned)blocks, BLOCK, 0, s>>>(
-        ws.spans, ws.pos[at], (const T *)dout, ws.part1, ws.part2, (W *)dw,
+        ws.spans, ws.pos[at], (const T *)dout, ws.part1, part2, (W *)dw,
         units, H, slices, scale);
     return hipGetLastError();
 }
@@ -478,35 +675,45 @@ hipError_t kf_embed_bwd(const void *ids, int wide, const void *dout,
     if (!fits(N, V, H)) return hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
     const Workspace ws((char *)work, N, V, H);
-    const int nb = (int)(N / SORT_TILE + 1);
+    const int nb = (int)((N + SORT_TILE - 1) / SORT_TILE);
     int bits = 1;
     while (V >> bits) ++bits;  // keys run to V itself
     const int passes = (bits + MAX_BITS - 1) / MAX_BITS;
     const int per = (bits + passes - 1) / passes;
-    for (int p = 0; p < passes; ++p) {
-        const int to = p % 2, from = 1 - to;
-        if (p == 0) {
-            sort_hist<true><<<nb, BLOCK, 0, s>>>(ids, wide, N, V, padding, 0,
-                                                 per, ws.hist, nb, ws.spans);
-        } else {
-            sort_hist<false><<<nb, BLOCK, 0, s>>>(ws.keys[from], 0, N, V,
-                                                  padding, p * per, per,
-                                                  ws.hist, nb, ws.spans);
+    // blocks beside those that sort, to clear the spans 16 ints a thread
+    const long long clear = 2 * V / (16 * BLOCK) + 1;
+    int at = 0;
+    if (N <= SMALL) {
+        const long long n = clear * BLOCK / SMALL_BLOCK + 1;
+        sort_small<<<1 + (unsigned)(n < 256 ? n : 256), SMALL_BLOCK, 0,
+                     s>>>(ids, wide, (int)N, V, padding, passes, per,
+                          ws.keys[0], ws.pos[0], ws.spans);
+    } else {
+        const bool scan = nb > SELF_SCAN;
+        for (int p = 0; p < passes; ++p) {
+            const int to = p % 2, from = 1 - to;
+            if (p == 0) {
+                const long long most = clear < 1024 ? clear : 1024;
+                sort_hist<true>
+                    <<<nb > most ? nb : (unsigned)most, BLOCK, 0, s>>>(
+                        ids, wide, N, V, padding, 0, per, ws.hist, nb,
+                        ws.spans);
+            } else {
+                sort_hist<false><<<nb, BLOCK, 0, s>>>(
+                    ws.keys[from], 0, N, V, padding, p * per, per, ws.hist,
+                    nb, nullptr);
+            }
+            if (scan) sort_scan<<<1, 1024, 0, s>>>(ws.hist, nb << per);
+            auto scatter = p == 0 ? (scan ? sort_scatter<true, true>
+                                          : sort_scatter<true, false>)
+                                  : (scan ? sort_scatter<false, true>
+                                          : sort_scatter<false, false>);
+            scatter<<<nb, BLOCK, 0, s>>>(
+                p == 0 ? ids : ws.keys[from], wide, ws.pos[from], N, V,
+                padding, p * per, per, ws.hist, nb, ws.keys[to], ws.pos[to]);
+            at = to;
         }
-        sort_scan<<<1, 1024, 0, s>>>(ws.hist, nb << per);
-        if (p == 0)
-            sort_scatter<true><<<nb, BLOCK, 0, s>>>(
-                ids, wide, nullptr, N, V, padding, 0, per, ws.hist, nb,
-                ws.keys[to], ws.pos[to]);
-        else
-            sort_scatter<false><<<nb, BLOCK, 0, s>>>(
-                ws.keys[from], 0, ws.pos[from], N, V, padding, p * per, per,
-                ws.hist, nb, ws.keys[to], ws.pos[to]);
     }
-    const int at = (passes - 1) % 2;
-    if (N)
-        token_bounds<<<(unsigned)((N + BLOCK - 1) / BLOCK), BLOCK, 0, s>>>(
-            ws.keys[at], N, (unsigned)V, ws.spans);
 #define CASE(WT, WI, OT, OI)                                                \
     if (wtype == WI && otype == OI)                                         \
     return sums_vec<OT, WT>(ws, at, dout, dw, N, V, H, scale, s)

@@ -58,7 +58,7 @@ hipError_t kf_embed_fwd(const void *, int, const void *, long long, int,
 hipError_t kf_embed_bwd(const void *, int, const void *, int, void *, int,
                         long long, long long, int, long long, float, void *,
                         void *);
-long long kf_qk_ws(int);
+long long kf_qk_ws(int, int);
 hipError_t kf_qk_norm_rope(const uintptr_t *, const long long *, int, float,
                            int, void *);
 long long kf_attn_ws(const long long *, int);
@@ -326,7 +326,7 @@ PYBIND11_MODULE(_hip, m)
           });
 
     // ---- query/key norm for each head with the position rotation ----
-    m.def("qk_ws", [](int D) { return kf_qk_ws(D); });
+    m.def("qk_ws", [](int D, int heads) { return kf_qk_ws(D, heads); });
     m.def("qk_norm_rope",
           [](const Ptrs &ptrs, const Dims &dims, int dtype, float eps,
              bool backward, uintptr_t stream) {
@@ -344,7 +344,7 @@ PYBIND11_MODULE(_hip, m)
     m.def("attn_fwd",
           [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
              float scale, int dtype, uintptr_t stream) {
-              check(kf_attn_fwd(list(ptrs, 8, "attn_fwd"),
+              check(kf_attn_fwd(list(ptrs, 9, "attn_fwd"),
                                 list(dims, 9, "attn_fwd"),
                                 list(strides, 9, "attn_fwd"), scale, dtype,
                                 (void *)stream),
@@ -353,7 +353,7 @@ PYBIND11_MODULE(_hip, m)
     m.def("attn_bwd",
           [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
              float scale, int dtype, uintptr_t stream) {
-              check(kf_attn_bwd(list(ptrs, 12, "attn_bwd"),
+              check(kf_attn_bwd(list(ptrs, 13, "attn_bwd"),
                                 list(dims, 9, "attn_bwd"),
                                 list(strides, 12, "attn_bwd"), scale, dtype,
                                 (void *)stream),

@@ -14,9 +14,13 @@
 // Both are bound by memory: forward reads x and writes y once, backward
 // reads x and dy and writes dx once. A row is held by L = D/16 lanes
 // (rounded up to a power of two) with eight pairs each, so the rotation
-// needs no exchange between lanes and the norm log2(L) shuffles. The rows
-// of a wave are heads of one token: their angles are the same cache lines,
-// read once and kept in registers over the heads.
+// needs no exchange between lanes and the norm log2(L) shuffles.
+//
+// A group of L lanes keeps one head and walks over the tokens, neighbouring
+// groups are neighbouring heads of a token: what a group needs of the
+// weights, and its sum of their gradient, stays in registers; the heads
+// share the cache lines of their token's angles; and the group has the rows
+// of several tokens on their way at once.
 #include "vec.hpp"
 
 using namespace kfv;
@@ -24,7 +28,6 @@ using namespace kfv;
 namespace {
 
 constexpr int BLOCK = 256;
-constexpr int WAVES = BLOCK / WAVE;
 constexpr int MAX_D = 512;
 
 struct Rows {          // [B][S][heads][D], last dimension dense
@@ -43,41 +46,55 @@ struct Args {
     long long pb, ps;
     int pwide;
     long long start, P;
-    long long tokens;
-    int S, D, lanes, lanes_log, wf32;
+    int tokens, S, D, lanes, lanes_log, wf32;
     float eps;
-    int split, heads_per;   // waves that share a token, heads of each
-    float *partial;         // backward: [blocks][2][D]
+    int groups, tstep;  // that have a head; tokens from one to the next
+    float *partial;     // backward: [blocks][2][D]
 };
 
-template <typename T, bool VEC>
-__device__ inline void load_pairs(float *lo, float *hi, const T *row, int D,
-                                  int li, int L)
+// Eight pairs of a row, columns li * 8 + j (VEC) or j * L + li; columns
+// past the last pair repeat one and are dropped.
+template <bool VEC>
+__device__ inline int pair_col(int li, int j, int L)
 {
-    const int half = D / 2;
-    if (VEC) {
-        if (li * 8 < half) {
-            ld8<T>(lo, row + li * 8);
-            ld8<T>(hi, row + half + li * 8);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 0.f;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = j * L + li;
-            lo[j] = i < half ? (float)row[i] : 0.f;
-            hi[j] = i < half ? (float)row[half + i] : 0.f;
-        }
-    }
+    return VEC ? li * 8 + j : j * L + li;
 }
 
 template <typename T, bool VEC>
+struct Pairs {
+    typename vec8<T>::type lo, hi;
+    __device__ void load(const T *row, int half, int li, int L)
+    {
+        if (VEC) {
+            const int c = li * 8 < half ? li * 8 : 0;
+            lo = *(const typename vec8<T>::type *)(row + c);
+            hi = *(const typename vec8<T>::type *)(row + half + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                int c = pair_col<VEC>(li, j, L);
+                c = c < half ? c : 0;
+                lo[j] = row[c];
+                hi[j] = row[half + c];
+            }
+        }
+    }
+    // as f32; zeros past the last pair
+    __device__ void get(float *l, float *h, int half, int li, int L) const
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = (VEC ? li * 8 : pair_col<VEC>(li, j, L)) < half;
+            l[j] = in ? (float)lo[j] : 0.f;
+            h[j] = in ? (float)hi[j] : 0.f;
+        }
+    }
+};
+
+template <typename T, bool VEC>
 __device__ inline void store_pairs(T *row, const float *lo, const float *hi,
-                                   int D, int li, int L)
+                                   int half, int li, int L)
 {
-    const int half = D / 2;
     if (VEC) {
         if (li * 8 < half) {
             st8<T>(row + li * 8, lo);
@@ -86,7 +103,7 @@ __device__ inline void store_pairs(T *row, const float *lo, const float *hi,
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int i = j * L + li;
+            const int i = pair_col<VEC>(li, j, L);
             if (i < half) {
                 row[i] = (T)lo[j];
                 row[half + i] = (T)hi[j];
@@ -97,44 +114,20 @@ __device__ inline void store_pairs(T *row, const float *lo, const float *hi,
 
 template <typename T, bool VEC>
 __device__ inline void load_weight(float *lo, float *hi, const void *w,
-                                   int wf32, int D, int li, int L)
+                                   int wf32, int half, int li, int L)
 {
     if (!w) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 1.f;
     } else if (wf32) {
-        load_pairs<float, VEC>(lo, hi, (const float *)w, D, li, L);
+        Pairs<float, VEC> p;
+        p.load((const float *)w, half, li, L);
+        p.get(lo, hi, half, li, L);
     } else {
-        load_pairs<T, VEC>(lo, hi, (const T *)w, D, li, L);
+        Pairs<T, VEC> p;
+        p.load((const T *)w, half, li, L);
+        p.get(lo, hi, half, li, L);
     }
-}
-
-// cos and sin of this lane's pairs at token (b, s). A position outside the
-// table is not followed: its angles, and so its rows, are NaN.
-template <bool VEC>
-__device__ inline void load_angles(float *cs, float *sn, const Args &a,
-                                   int b, int s, int li)
-{
-    if (!a.rope) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            cs[j] = 1.f;
-            sn[j] = 0.f;
-        }
-        return;
-    }
-    long long pos = a.start + s;
-    if (a.positions) {
-        const long long at = b * a.pb + s * a.ps;
-        pos = a.pwide ? ((const long long *)a.positions)[at]
-                      : (long long)((const int *)a.positions)[at];
-    }
-    if (pos < 0 || pos >= a.P) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cs[j] = sn[j] = __builtin_nanf("");
-        return;
-    }
-    load_pairs<float, VEC>(cs, sn, a.rope + pos * a.D, a.D, li, a.lanes);
 }
 
 __device__ inline float group_sum(float v, int L)
@@ -143,201 +136,251 @@ __device__ inline float group_sum(float v, int L)
     return v;
 }
 
-template <typename T, bool VEC>
-__device__ inline void fwd_rows(const Args &a, const Rows &x, int b, int s,
-                                long long token, int h0, int h1, int li,
-                                int gi, const float *cs, const float *sn)
-{
-    const int L = a.lanes, per = WAVE >> a.lanes_log;
-    float wl[8], wh[8];
-    load_weight<T, VEC>(wl, wh, x.w, a.wf32, a.D, li, L);
-    for (int h = h0 + gi; h - gi < h1; h += per) {
-        const bool on = h < h1;
-        const T *row = (const T *)x.x + b * x.xb + s * x.xs +
-                       (long long)(on ? h : h0) * x.xh;
-        float lo[8], hi[8], yl[8], yh[8], q = 0.f;
-        load_pairs<T, VEC>(lo, hi, row, a.D, li, L);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q += lo[j] * lo[j] + hi[j] * hi[j];
-        const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float u = lo[j] * r * wl[j], v = hi[j] * r * wh[j];
-            yl[j] = u * cs[j] - v * sn[j];
-            yh[j] = v * cs[j] + u * sn[j];
+// A lane group's way over the tokens: its head, and where its rows of the
+// token it stands at begin. Past the last token it stands still.
+template <typename T, bool BWD>
+struct Walk {
+    int token, b, s;
+    const T *x, *dy;
+    T *out;
+    long long step_x, wrap_x, step_g, wrap_g, step_o;
+    bool is_q;
+    __device__ Walk(const Args &a, int gid)
+    {
+        const int all = a.q.heads + a.k.heads;
+        token = gid / all;
+        int h = gid - token * all;
+        if (gid >= a.groups) token = a.tokens;
+        is_q = h < a.q.heads;
+        const Rows &r = is_q ? a.q : a.k;
+        h = is_q ? h : h - a.q.heads;
+        const int t = token < a.tokens ? token : 0;
+        b = t / a.S;
+        s = t - b * a.S;
+        const int db = a.tstep / a.S, ds = a.tstep - db * a.S;
+        const long long xb = is_q ? a.q.xb : a.k.xb;
+        const long long xs = is_q ? a.q.xs : a.k.xs;
+        const long long xh = is_q ? a.q.xh : a.k.xh;
+        x = (const T *)(is_q ? a.q.x : a.k.x) + b * xb + s * xs + h * xh;
+        step_x = db * xb + ds * xs;
+        wrap_x = xb - a.S * xs;
+        const int heads = is_q ? a.q.heads : a.k.heads;
+        out = (T *)(is_q ? a.q.out : a.k.out) +
+              ((long long)t * heads + h) * a.D;
+        step_o = (long long)a.tstep * heads * a.D;
+        if (BWD) {
+            const long long gb = is_q ? a.q.gb : a.k.gb;
+            const long long gs = is_q ? a.q.gs : a.k.gs;
+            const long long gh = is_q ? a.q.gh : a.k.gh;
+            dy = (const T *)(is_q ? a.q.dy : a.k.dy) + b * gb + s * gs +
+                 h * gh;
+            step_g = db * gb + ds * gs;
+            wrap_g = gb - a.S * gs;
         }
-        if (on)
-            store_pairs<T, VEC>((T *)x.out + (token * x.heads + h) * a.D, yl,
-                                yh, a.D, li, L);
     }
-}
+    __device__ bool on(const Args &a) const { return token < a.tokens; }
+    __device__ void next(const Args &a)
+    {
+        if (token < a.tokens - a.tstep) {
+            const int db = a.tstep / a.S, ds = a.tstep - db * a.S;
+            b += db;
+            s += ds;
+            x += step_x;
+            out += step_o;
+            if (BWD) dy += step_g;
+            if (s >= a.S) {
+                s -= a.S;
+                b += 1;
+                x += wrap_x;
+                if (BWD) dy += wrap_g;
+            }
+            token += a.tstep;
+        } else {
+            token = a.tokens;
+        }
+    }
+    // Row of the table; -1 for a position outside it, which is not
+    // followed: its rows are NaN.
+    __device__ long long position(const Args &a) const
+    {
+        long long pos = a.start + s;
+        if (a.positions) {
+            const long long at = b * a.pb + s * a.ps;
+            pos = a.pwide ? ((const long long *)a.positions)[at]
+                          : (long long)((const int *)a.positions)[at];
+        }
+        return pos < 0 || pos >= a.P ? -1 : pos;
+    }
+};
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(BLOCK) void qk_fwd(Args a)
+struct Angles {
+    Pairs<float, VEC> p;
+    bool ok;
+    template <typename W>
+    __device__ void load(const Args &a, const W &w, int li)
+    {
+        if (!a.rope) return;
+        const long long pos = w.position(a);
+        ok = pos >= 0;
+        p.load(a.rope + (ok ? pos : 0) * a.D, a.D / 2, li, a.lanes);
+    }
+    __device__ void get(float *cs, float *sn, const Args &a) const
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            cs[j] = !a.rope ? 1.f : ok ? p.lo[j] : __builtin_nanf("");
+            sn[j] = !a.rope ? 0.f : ok ? p.hi[j] : __builtin_nanf("");
+        }
+    }
+};
+
+// U tokens at a time: their loads go out together.
+template <typename T, bool VEC, int U>
+__global__ __launch_bounds__(BLOCK) void qk_fwd(const Args a)
 {
     const int lane = threadIdx.x % WAVE;
-    const int li = lane & (a.lanes - 1), gi = lane >> a.lanes_log;
-    const int all = a.q.heads + a.k.heads;
-    const long long units = a.tokens * a.split;
-    for (long long u = (long long)blockIdx.x * WAVES + threadIdx.x / WAVE;
-         u < units; u += (long long)gridDim.x * WAVES) {
-        const int token =
-            __builtin_amdgcn_readfirstlane((int)(u / a.split));
-        const int part =
-            __builtin_amdgcn_readfirstlane((int)(u - (long long)token *
-                                                         a.split));
-        const int b = token / a.S, s = token - b * a.S;
-        float cs[8], sn[8];
-        load_angles<VEC>(cs, sn, a, b, s, li);
-        const int h0 = part * a.heads_per;
-        const int h1 = h0 + a.heads_per < all ? h0 + a.heads_per : all;
-        if (h0 < a.q.heads)
-            fwd_rows<T, VEC>(a, a.q, b, s, token, h0,
-                             h1 < a.q.heads ? h1 : a.q.heads, li, gi, cs,
-                             sn);
-        if (h1 > a.q.heads)
-            fwd_rows<T, VEC>(a, a.k, b, s, token,
-                             h0 > a.q.heads ? h0 - a.q.heads : 0,
-                             h1 - a.q.heads, li, gi, cs, sn);
-    }
-}
-
-template <typename T, bool VEC>
-__device__ inline void bwd_rows(const Args &a, const Rows &x, int b, int s,
-                                long long token, int h0, int h1, int li,
-                                int gi, const float *cs, const float *sn,
-                                const float *wl, const float *wh, float *al,
-                                float *ah)
-{
-    const int L = a.lanes, per = WAVE >> a.lanes_log;
-    for (int h = h0 + gi; h - gi < h1; h += per) {
-        const bool on = h < h1;
-        const long long hh = on ? h : h0;
-        float lo[8], hi[8], gl[8], gh[8], q = 0.f, t = 0.f;
-        load_pairs<T, VEC>(lo, hi,
-                           (const T *)x.x + b * x.xb + s * x.xs + hh * x.xh,
-                           a.D, li, L);
-        load_pairs<T, VEC>(gl, gh,
-                           (const T *)x.dy + b * x.gb + s * x.gs + hh * x.gh,
-                           a.D, li, L);
+    const int L = a.lanes, li = lane & (L - 1), half = a.D / 2;
+    Walk<T, false> w(a, (blockIdx.x * BLOCK + threadIdx.x) >> a.lanes_log);
+    float wl[8], wh[8];
+    load_weight<T, VEC>(wl, wh, w.is_q ? a.q.w : a.k.w, a.wf32, half, li, L);
+    const int turns = (a.tokens + a.tstep - 1) / a.tstep;
+    for (int turn = 0; turn < turns; turn += U) {
+        Pairs<T, VEC> x[U];
+        Angles<T, VEC> ang[U];
+        T *out[U];
+        bool on[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            q += lo[j] * lo[j] + hi[j] * hi[j];
-            const float u = gl[j] * cs[j] + gh[j] * sn[j];
-            const float v = gh[j] * cs[j] - gl[j] * sn[j];
-            gl[j] = u;
-            gh[j] = v;
-            t += u * wl[j] * lo[j] + v * wh[j] * hi[j];
+        for (int u = 0; u < U; ++u) {
+            on[u] = w.on(a);
+            out[u] = w.out;
+            x[u].load(w.x, half, li, L);
+            ang[u].load(a, w, li);
+            w.next(a);
         }
-        const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
-        const float m = group_sum(t, L) / (float)a.D * r * r * r;
-        if (on) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float lo[8], hi[8], cs[8], sn[8], q = 0.f;
+            x[u].get(lo, hi, half, li, L);
+            ang[u].get(cs, sn, a);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q += lo[j] * lo[j] + hi[j] * hi[j];
+            const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                al[j] += gl[j] * lo[j] * r;
-                ah[j] += gh[j] * hi[j] * r;
-                gl[j] = gl[j] * wl[j] * r - lo[j] * m;
-                gh[j] = gh[j] * wh[j] * r - hi[j] * m;
+                const float c = lo[j] * r * wl[j], d = hi[j] * r * wh[j];
+                lo[j] = c * cs[j] - d * sn[j];
+                hi[j] = d * cs[j] + c * sn[j];
             }
-            store_pairs<T, VEC>((T *)x.out + (token * x.heads + h) * a.D, gl,
-                                gh, a.D, li, L);
+            if (on[u]) store_pairs<T, VEC>(out[u], lo, hi, half, li, L);
         }
     }
 }
 
-// Adds the row groups of every wave of the block in a fixed order and
-// writes the block's sum of one weight's gradient.
-template <bool VEC>
-__device__ inline void block_weight(const float *al, const float *ah,
-                                    float *lds, float *dst, int D, int li,
-                                    int gi, int L, int per, int wid)
+template <typename T, bool VEC, int U>
+__global__ __launch_bounds__(BLOCK) void qk_bwd(const Args a)
 {
-    const int half = D / 2;
-    __syncthreads();
-    float *mine = lds + wid * D;
-    for (int g = 0; g < per; ++g) {  // a wave's groups, one after another
-        if (g == gi) {
+    __shared__ float lds[BLOCK * 16];  // [groups][D]
+    const int lane = threadIdx.x % WAVE;
+    const int L = a.lanes, li = lane & (L - 1), half = a.D / 2;
+    Walk<T, true> w(a, (blockIdx.x * BLOCK + threadIdx.x) >> a.lanes_log);
+    float wl[8], wh[8], al[8] = {}, ah[8] = {};
+    load_weight<T, VEC>(wl, wh, w.is_q ? a.q.w : a.k.w, a.wf32, half, li, L);
+    const int turns = (a.tokens + a.tstep - 1) / a.tstep;
+    for (int turn = 0; turn < turns; turn += U) {
+        Pairs<T, VEC> x[U], dy[U];
+        Angles<T, VEC> ang[U];
+        T *out[U];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            on[u] = w.on(a);
+            out[u] = w.out;
+            x[u].load(w.x, half, li, L);
+            dy[u].load(w.dy, half, li, L);
+            ang[u].load(a, w, li);
+            w.next(a);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float lo[8], hi[8], gl[8], gh[8], cs[8], sn[8];
+            float q = 0.f, t = 0.f;
+            x[u].get(lo, hi, half, li, L);
+            dy[u].get(gl, gh, half, li, L);
+            ang[u].get(cs, sn, a);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int i = VEC ? li * 8 + j : j * L + li;
-                if (i < half) {
-                    mine[i] = (g ? mine[i] : 0.f) + al[j];
-                    mine[half + i] = (g ? mine[half + i] : 0.f) + ah[j];
+                q += lo[j] * lo[j] + hi[j] * hi[j];
+                const float c = gl[j] * cs[j] + gh[j] * sn[j];
+                const float d = gh[j] * cs[j] - gl[j] * sn[j];
+                gl[j] = c;
+                gh[j] = d;
+                t += c * wl[j] * lo[j] + d * wh[j] * hi[j];
+            }
+            const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
+            const float m = group_sum(t, L) / (float)a.D * r * r * r;
+            if (on[u]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    al[j] += gl[j] * lo[j] * r;
+                    ah[j] += gh[j] * hi[j] * r;
+                    gl[j] = gl[j] * wl[j] * r - lo[j] * m;
+                    gh[j] = gh[j] * wh[j] * r - hi[j] * m;
                 }
+                store_pairs<T, VEC>(out[u], gl, gh, half, li, L);
             }
         }
-        __syncthreads();
     }
-    for (int i = threadIdx.x; i < D; i += BLOCK) {
+    if (!a.partial) return;
+    // the block's sums: its groups' in order, q's and k's apart
+    const int g = threadIdx.x >> a.lanes_log;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int i = pair_col<VEC>(li, j, L);
+        if (i < half) {
+            lds[g * a.D + i] = al[j];
+            lds[g * a.D + half + i] = ah[j];
+        }
+    }
+    __syncthreads();
+    const int all = a.q.heads + a.k.heads, groups = BLOCK >> a.lanes_log;
+    const int h0 = (int)((long long)blockIdx.x * groups % all);
+    float *dst = a.partial + (long long)blockIdx.x * 2 * a.D;
+    for (int i = threadIdx.x; i < 2 * a.D; i += BLOCK) {
+        const bool want_q = i < a.D;
+        const int c = want_q ? i : i - a.D;
         float v = 0.f;
-        for (int w = 0; w < WAVES; ++w) v += lds[w * D + i];
+        for (int k = 0, h = h0; k < groups; ++k) {
+            if ((h < a.q.heads) == want_q) v += lds[k * a.D + c];
+            h = h + 1 < all ? h + 1 : 0;
+        }
         dst[i] = v;
     }
 }
 
-template <typename T, bool VEC>
-__global__ __launch_bounds__(BLOCK) void qk_bwd(Args a)
-{
-    __shared__ float lds[WAVES * MAX_D];
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
-    const int li = lane & (a.lanes - 1), gi = lane >> a.lanes_log;
-    const int all = a.q.heads + a.k.heads;
-    const long long units = a.tokens * a.split;
-    float qwl[8], qwh[8], kwl[8], kwh[8];
-    float ql[8] = {}, qh[8] = {}, kl[8] = {}, kh[8] = {};
-    load_weight<T, VEC>(qwl, qwh, a.q.w, a.wf32, a.D, li, a.lanes);
-    load_weight<T, VEC>(kwl, kwh, a.k.w, a.wf32, a.D, li, a.lanes);
-    for (long long u = (long long)blockIdx.x * WAVES + wid; u < units;
-         u += (long long)gridDim.x * WAVES) {
-        const int token =
-            __builtin_amdgcn_readfirstlane((int)(u / a.split));
-        const int part =
-            __builtin_amdgcn_readfirstlane((int)(u - (long long)token *
-                                                         a.split));
-        const int b = token / a.S, s = token - b * a.S;
-        float cs[8], sn[8];
-        load_angles<VEC>(cs, sn, a, b, s, li);
-        const int h0 = part * a.heads_per;
-        const int h1 = h0 + a.heads_per < all ? h0 + a.heads_per : all;
-        if (h0 < a.q.heads)
-            bwd_rows<T, VEC>(a, a.q, b, s, token, h0,
-                             h1 < a.q.heads ? h1 : a.q.heads, li, gi, cs,
-                             sn, qwl, qwh, ql, qh);
-        if (h1 > a.q.heads)
-            bwd_rows<T, VEC>(a, a.k, b, s, token,
-                             h0 > a.q.heads ? h0 - a.q.heads : 0,
-                             h1 - a.q.heads, li, gi, cs, sn, kwl, kwh, kl,
-                             kh);
-    }
-    if (a.partial) {
-        float *dst = a.partial + (long long)blockIdx.x * 2 * a.D;
-        const int per = WAVE >> a.lanes_log;
-        block_weight<VEC>(ql, qh, lds, dst, a.D, li, gi, a.lanes, per, wid);
-        block_weight<VEC>(kl, kh, lds, dst + a.D, a.D, li, gi, a.lanes, per,
-                          wid);
-    }
-}
-
-// dw[c] = sum of the blocks' partial sums, 64 columns a block: wave w adds
-// every fourth partial, the four sums are added in order.
+// dw[c] = sum of the blocks' partial sums, 64 columns a block: each of 16
+// waves adds every 16th partial, the waves' sums are added in order.
+constexpr int WBLOCK = 1024;
 template <typename T>
-__global__ __launch_bounds__(BLOCK) void qk_weight(
+__global__ __launch_bounds__(WBLOCK) void qk_weight(
     const float *__restrict__ partial, int blocks, int D, int wf32,
     void *__restrict__ dqw, void *__restrict__ dkw)
 {
-    __shared__ float lds[WAVES][WAVE];
+    constexpr int NW = WBLOCK / WAVE;
+    __shared__ float lds[NW][WAVE];
     const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
     const int c = blockIdx.x * WAVE + lane;
     float v = 0.f;
     if (c < 2 * D) {
-#pragma unroll 8
-        for (int i = wid; i < blocks; i += WAVES)
+#pragma unroll 16
+        for (int i = wid; i < blocks; i += NW)
             v += partial[(long long)i * 2 * D + c];
     }
     lds[wid][lane] = v;
     __syncthreads();
     if (wid == 0 && c < 2 * D) {
-        v = lds[0][lane] + lds[1][lane] + lds[2][lane] + lds[3][lane];
+        v = 0.f;
+        for (int i = 0; i < NW; ++i) v += lds[i][lane];
         void *dw = c < D ? dqw : dkw;
         const int i = c < D ? c : c - D;
         if (dw) {
@@ -363,53 +406,55 @@ bool vec_ok(const Args &a, bool backward)
     return ok;
 }
 
-// Heads of a token are shared by as many waves as keep four rows for each
-// lane group, evenly.
-void shape(Args &a)
+constexpr int FWD_U = 4, BWD_U = 2;  // rows of a group on their way
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
+
+// Lanes of a row, and blocks: a group for each head of as many tokens as
+// leave each group U rows, up to as many blocks as the chip holds.
+int shape(Args &a, int U, int most)
 {
-    const int groups = (a.D / 2 + 7) / 8;
+    const int need = (a.D / 2 + 7) / 8;
     a.lanes = 1;
     a.lanes_log = 0;
-    while (a.lanes < groups) {
+    while (a.lanes < need) {
         a.lanes *= 2;
         a.lanes_log += 1;
     }
-    const int all = a.q.heads + a.k.heads;
-    const int most = 4 * (WAVE / a.lanes);
-    a.split = (all + most - 1) / most;
-    a.heads_per = (all + a.split - 1) / a.split;
-}
-
-constexpr int BWD_BLOCKS = 512;
-
-long long blocks_of(const Args &a)
-{
-    return (a.tokens * a.split + WAVES - 1) / WAVES;
+    const long long all = a.q.heads + a.k.heads;
+    const long long per = BLOCK / a.lanes;  // groups of a block
+    long long blocks =
+        (all * ((a.tokens + U - 1) / U) + per - 1) / per;
+    if (blocks > most) blocks = most;
+    const long long least = (all + per - 1) / per;
+    if (blocks < least) blocks = least;
+    long long tstep = blocks * per / all;
+    if (tstep > a.tokens) tstep = a.tokens > 0 ? a.tokens : 1;
+    a.tstep = (int)tstep;
+    a.groups = (int)(tstep * all);
+    return (int)blocks;
 }
 
 template <typename T>
 hipError_t launch(Args &a, bool backward, void *dqw, void *dkw,
                   hipStream_t s)
 {
-    long long blocks = blocks_of(a);
     const bool vec = vec_ok(a, backward);
     if (!backward) {
-        if (blocks > 1 << 20) blocks = 1 << 20;
+        const int blocks = shape(a, FWD_U, FWD_BLOCKS);
         if (vec)
-            qk_fwd<T, true><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+            qk_fwd<T, true, FWD_U><<<blocks, BLOCK, 0, s>>>(a);
         else
-            qk_fwd<T, false><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+            qk_fwd<T, false, FWD_U><<<blocks, BLOCK, 0, s>>>(a);
         return hipGetLastError();
     }
-    if (blocks > BWD_BLOCKS) blocks = BWD_BLOCKS;
-    if (blocks < 1) blocks = 1;  // no tokens: the weights' zeros
+    const int blocks = shape(a, BWD_U, BWD_BLOCKS);
     if (vec)
-        qk_bwd<T, true><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+        qk_bwd<T, true, BWD_U><<<blocks, BLOCK, 0, s>>>(a);
     else
-        qk_bwd<T, false><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+        qk_bwd<T, false, BWD_U><<<blocks, BLOCK, 0, s>>>(a);
     if (a.partial)
-        qk_weight<T><<<(2 * a.D + WAVE - 1) / WAVE, BLOCK, 0, s>>>(
-            a.partial, (int)blocks, a.D, a.wf32, dqw, dkw);
+        qk_weight<T><<<(2 * a.D + WAVE - 1) / WAVE, WBLOCK, 0, s>>>(
+            a.partial, blocks, a.D, a.wf32, dqw, dkw);
     return hipGetLastError();
 }
 
@@ -418,7 +463,14 @@ hipError_t launch(Args &a, bool backward, void *dqw, void *dkw,
 extern "C" {
 
 // floats of the backward's workspace
-long long kf_qk_ws(int D) { return (long long)BWD_BLOCKS * 2 * D; }
+long long kf_qk_ws(int D, int heads)
+{
+    Args a = {};
+    a.D = D;
+    a.q.heads = heads;
+    a.tokens = 1 << 30;
+    return (long long)shape(a, BWD_U, BWD_BLOCKS) * 2 * D;
+}
 
 // ptrs: q, k, qw, kw, out_q, out_k, rope, positions
 //       [, dyq, dyk, dqw, dkw, partial]
@@ -437,7 +489,12 @@ hipError_t kf_qk_norm_rope(const uintptr_t *ptrs, const long long *dims,
     a.k.out = (void *)ptrs[5];
     a.rope = (const float *)ptrs[6];
     a.positions = (const void *)ptrs[7];
-    a.tokens = dims[0];
+    if (dims[0] < 0 || dims[0] >= 1ll << 30 || dims[1] < 1 ||
+        dims[1] >= 1ll << 30 || dims[2] < 2 || dims[2] > MAX_D ||
+        dims[2] % 2 || dims[3] < 0 || dims[4] < 0 ||
+        dims[3] + dims[4] < 1 || dims[3] + dims[4] > 1 << 16)
+        return hipErrorInvalidValue;
+    a.tokens = (int)dims[0];
     a.S = (int)dims[1];
     a.D = (int)dims[2];
     a.q.heads = (int)dims[3];
@@ -469,12 +526,7 @@ hipError_t kf_qk_norm_rope(const uintptr_t *ptrs, const long long *dims,
         a.k.gs = dims[21];
         a.k.gh = dims[22];
     }
-    if (a.tokens < 0 || a.tokens >= 1ll << 30 || a.S < 1 || a.D < 2 ||
-        a.D % 2 || a.D > MAX_D || a.q.heads < 0 || a.k.heads < 0 ||
-        a.q.heads + a.k.heads < 1 || a.q.heads + a.k.heads > 1 << 16)
-        return hipErrorInvalidValue;
     if (a.tokens == 0 && !a.partial) return hipSuccess;
-    shape(a);
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
     case 0: return launch<float>(a, backward, dqw, dkw, s);

@@ -30,6 +30,10 @@ template <>
 struct vec8<_Float16> {
     typedef f16x8 type;
 };
+template <>
+struct vec8<float> {  // loaded as two pieces of 16 bytes
+    typedef __attribute__((ext_vector_type(8), aligned(16))) float type;
+};
 
 template <typename T>
 __device__ inline void ld8(float *f, const T *p)

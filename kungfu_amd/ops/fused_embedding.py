@@ -51,8 +51,7 @@ def _forward(ids, weight, scale, out_dtype):
     h = hip._require()
     w = weight if weight.stride(1) == 1 or weight.shape[1] == 1 else \
         weight.contiguous()
-    out = torch.empty(ids.shape + weight.shape[1:], dtype=out_dtype,
-                      device=weight.device)
+    out = weight.new_empty(ids.shape + weight.shape[1:], dtype=out_dtype)
     if ids.numel():
         with hip.on_device(weight):
             h.embed_fwd(ids.data_ptr(), ids.dtype == torch.int64,
@@ -75,12 +74,13 @@ class _Embedding(torch.autograd.Function):
         ids, = ctx.saved_tensors
         (V, H), dtype, scale, padding_idx, out_dtype = ctx.of
         h = hip._require()
-        dout = dout.to(out_dtype).contiguous()
-        dw = torch.empty((V, H), dtype=dtype, device=dout.device)
+        if dout.dtype != out_dtype:
+            dout = dout.to(out_dtype)
+        dout = dout.contiguous()
+        dw = dout.new_empty((V, H), dtype=dtype)
         N = ids.numel()
         with hip.on_device(dout):
-            ws = torch.empty(h.embed_ws(N, V, H), dtype=torch.uint8,
-                             device=dout.device)
+            ws = dout.new_empty(h.embed_ws(N, V, H), dtype=torch.uint8)
             h.embed_bwd(ids.data_ptr(), ids.dtype == torch.int64,
                         dout.data_ptr(), hip_dtype(out_dtype), dw.data_ptr(),
                         hip_dtype(dtype), N, V, H,

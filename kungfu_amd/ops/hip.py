@@ -214,13 +214,37 @@ def transform2(z, x, op="sum"):
 
 # ---- what the transformer ops share ----
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+# The current device and its stream as numbers, without the Python objects
+# around them, which cost as much as a small kernel.
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_now = getattr(
+    torch._C, "_cuda_getCurrentRawStream",
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def on_device(t):
     """Makes t's device current, for a launch on its stream."""
-    return torch.cuda.device(t.device)
+    index = t.get_device()
+    return _HERE if _device_now() == index else torch.cuda.device(index)
 
 
 def stream_of(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _stream_now(t.get_device())
+
+
+def dense_like(t):
+    """An uninitialised tensor of t's shape and type, row-major whatever
+    t's strides are."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def row_strides(t):

@@ -129,8 +129,7 @@ def _launch(q, k, qw, kw, oq, ok, rope, positions, start, eps, grads=None):
 
 
 def _forward(q, k, qw, kw, rope, positions, start, eps):
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    oq, ok = hip.dense_like(q), hip.dense_like(k)
     if oq.numel() or ok.numel():
         with hip.on_device(q):
             _launch(q, k, qw, kw, oq, ok, rope, positions, start, eps)
@@ -150,17 +149,16 @@ class _QKNormRope(torch.autograd.Function):
         q, k, qw, kw, rope, positions = ctx.saved_tensors
         start, eps = ctx.of
         dyq, dyk = _dense_rows(dyq), _dense_rows(dyk)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = hip.dense_like(q), hip.dense_like(k)
         dqw = None if qw is None else torch.empty_like(qw)
         dkw = None if kw is None else torch.empty_like(kw)
         partial = None
         if q.shape[2] + k.shape[2]:
             with hip.on_device(q):
                 if dqw is not None or dkw is not None:
-                    partial = torch.empty(
-                        hip._require().qk_ws(q.shape[3]),
-                        dtype=torch.float32, device=q.device)
+                    size = hip._require().qk_ws(
+                        q.shape[3], q.shape[2] + k.shape[2])
+                    partial = q.new_empty(size, dtype=torch.float32)
                 _launch(q, k, qw, kw, dq, dk, rope, positions, start, eps,
                         (dyq, dyk, dqw, dkw, partial))
         return dq, dk, dqw, dkw, None, None, None, None

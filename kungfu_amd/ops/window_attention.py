@@ -115,52 +115,52 @@ def _int32(t):
 
 
 def _forward(q, k, v, dims, lengths, starts, scale, keep):
+    """The output and, to keep for the backward, each row's log-sum-exp in
+    powers of two and what rounding took off the output."""
     h = hip._require()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = None
+    out = hip.dense_like(q)
+    lse = rest = None
     if keep:
-        lse = torch.empty(dims[0] * dims[1] * q.shape[2],
-                          dtype=torch.float32, device=q.device)
+        lse = q.new_empty(dims[0] * dims[1] * q.shape[2],
+                          dtype=torch.float32)
+        rest = hip.dense_like(q)
+    strides = [*hip.row_strides(q), *hip.row_strides(k),
+               *hip.row_strides(v)]
     with hip.on_device(q):
         size = h.attn_ws(dims, False)
-        ws = None
-        if size > 0:
-            ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(size, dtype=torch.uint8) if size > 0 else None
         h.attn_fwd([q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                    out.data_ptr(), _ptr(lse), _ptr(lengths), _ptr(starts),
-                    _ptr(ws)], dims,
-                   [*hip.row_strides(q), *hip.row_strides(k),
-                    *hip.row_strides(v)], scale, hip_dtype(q.dtype),
-                   hip.stream_of(q))
-    return out, lse
+                    out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(lengths),
+                    _ptr(starts), _ptr(ws)], dims, strides, scale,
+                   hip_dtype(q.dtype), hip.stream_of(q))
+    return out, lse, rest, strides
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, dims, lengths, starts, scale):
-        out, lse = _forward(q, k, v, dims, lengths, starts, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths, starts)
-        ctx.of = (dims, scale)
+        out, lse, rest, strides = _forward(q, k, v, dims, lengths, starts,
+                                           scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, rest, lengths, starts)
+        ctx.of = (dims, scale, strides)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths, starts = ctx.saved_tensors
-        dims, scale = ctx.of
+        q, k, v, out, lse, rest, lengths, starts = ctx.saved_tensors
+        dims, scale, strides = ctx.of
         h = hip._require()
         dout = hip.rows16(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                      for t in (q, k, v))
+        dq, dk, dv = hip.dense_like(q), hip.dense_like(k), hip.dense_like(v)
         with hip.on_device(q):
-            ws = torch.empty(h.attn_ws(dims, True), dtype=torch.uint8,
-                             device=q.device)
+            ws = q.new_empty(h.attn_ws(dims, True), dtype=torch.uint8)
             h.attn_bwd([q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                        out.data_ptr(), lse.data_ptr(), _ptr(lengths),
-                        _ptr(starts), dout.data_ptr(), dq.data_ptr(),
-                        dk.data_ptr(), dv.data_ptr(), ws.data_ptr()], dims,
-                       [*hip.row_strides(q), *hip.row_strides(k),
-                        *hip.row_strides(v), *hip.row_strides(dout)], scale,
+                        out.data_ptr(), lse.data_ptr(), rest.data_ptr(),
+                        _ptr(lengths), _ptr(starts), dout.data_ptr(),
+                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                        ws.data_ptr()], dims,
+                       strides + hip.row_strides(dout), scale,
                        hip_dtype(q.dtype), hip.stream_of(q))
         return dq, dk, dv, None, None, None, None
 
