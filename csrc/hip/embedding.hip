@@ -22,9 +22,9 @@ constexpr int BLOCK = 256;
 constexpr int WAVES = BLOCK / WAVE;
 constexpr int MAX_BITS = 8;               // digit bits of one pass
 constexpr int MAX_DIGITS = 1 << MAX_BITS;
-constexpr int SORT_TILE = 2048;           // keys a block ranks in one pass
+constexpr int SORT_TILE = 1024;           // keys a block ranks in one pass
 constexpr int SORT_ROUNDS = SORT_TILE / BLOCK;
-constexpr int SELF_SCAN = 64;  // blocks up to which each finds its own places
+constexpr int SELF_SCAN = 128; // blocks up to which each finds its own places
 constexpr int SMALL = 8192;    // keys up to which one block sorts them all
 constexpr int SMALL_BLOCK = 1024;
 constexpr int CHUNK = 32;                 // rows that one partial sum joins
@@ -501,12 +501,16 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
                 const int here = CHUNK - i % CHUNK;
                 int n = here < left ? here : left;
                 n = n < 8 ? n : 8;
-                if (n == 1)
-                    add_rows<T, C, 1>(acc, dout, 1, c0, lane, H,
-                                      [&](int) { return pos[i]; });
+                // no more loads than twice the rows that are there
+                auto row = [&](int k) { return pos[i + k]; };
+                if (n > 4)
+                    add_rows<T, C, 8>(acc, dout, n, c0, lane, H, row);
+                else if (n > 2)
+                    add_rows<T, C, 4>(acc, dout, n, c0, lane, H, row);
+                else if (n > 1)
+                    add_rows<T, C, 2>(acc, dout, n, c0, lane, H, row);
                 else
-                    add_rows<T, C, 8>(acc, dout, n, c0, lane, H,
-                                      [&](int k) { return pos[i + k]; });
+                    add_rows<T, C, 1>(acc, dout, n, c0, lane, H, row);
                 i += n;
             } else if (!part2 || i % BIG || left < BIG) {
                 // up to the next chunk of chunks, or to the last chunk

@@ -406,8 +406,8 @@ bool vec_ok(const Args &a, bool backward)
     return ok;
 }
 
-constexpr int FWD_U = 4, BWD_U = 2;  // rows of a group on their way
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
+constexpr int FWD_U = 2, BWD_U = 2;  // rows of a group on their way
+constexpr int FWD_BLOCKS = 1024, BWD_BLOCKS = 512;
 
 // Lanes of a row, and blocks: a group for each head of as many tokens as
 // leave each group U rows, up to as many blocks as the chip holds.

@@ -428,16 +428,22 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     const int wp0 = s.start + w0 / a.G;
     const int wp1 = w0 < SG ? s.start + wlast / a.G : INT_MIN / 2;
 
+    // loads are not branched around, which would wait for each: lanes
+    // without a row, or past the last column, read others and drop them
     s16x8 qop[DP / 16];
     {
-        const short *row = (const short *)a.q + b * a.qb + qi * a.qs +
-                           (long long)(h * a.G + g) * a.qh;
+        const int rr = r < SG ? r : SG - 1, i = rr / a.G, gg = rr - i * a.G;
+        const short *row = (const short *)a.q + b * a.qb + i * a.qs +
+                           (long long)(h * a.G + gg) * a.qh;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             const int d = i * 16 + lane / 32 * 8;
-            s16x8 x = {};
-            if (live && d < a.D) x = *(const s16x8 *)(row + d);
-            qop[i] = x;
+            qop[i] = *(const s16x8 *)(row + (d < a.D ? d : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int d = i * 16 + lane / 32 * 8;
+            if (!live || d >= a.D) qop[i] = s16x8{};
         }
     }
 
@@ -547,8 +553,11 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         // the places that follow from these two are worked out again: kept,
         // they would take the registers of half a tile's scores
         asm volatile("" : "+v"(rat), "+v"(cat));
+        // before waves that settle: 881 -> 913 TFLOP/s at 64 columns
+        __builtin_amdgcn_s_setprio(1);
         score(kt, x);
         weigh(vt, xp);
+        __builtin_amdgcn_s_setprio(0);
         settle(tl.at(i) * KT, x);
         ++i;
     };
@@ -699,30 +708,33 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
     s16x8 qop[DP / 16], gop[DP / 16];
     float delta = 0.f;
     {
-        const short *qrow = (const short *)a.q + b * a.qb + qi * a.qs +
-                            (long long)head * a.qh;
-        const short *grow = (const short *)a.dout + b * a.gb + qi * a.gs +
-                            (long long)head * a.gh;
-        const T *out = (const T *)a.o + orow;
-        const T *rest = (const T *)a.orest + orow;
+        const int rr = r < SG ? r : SG - 1, i = rr / a.G;
+        const int hh = h * a.G + rr - i * a.G;
+        const short *qrow = (const short *)a.q + b * a.qb + i * a.qs +
+                            (long long)hh * a.qh;
+        const short *grow = (const short *)a.dout + b * a.gb + i * a.gs +
+                            (long long)hh * a.gh;
+        const long long at =
+            (((long long)b * a.S + i) * a.Hk * a.G + hh) * a.D;
+        typedef typename vec8<T>::type T8;
+        T8 o[DP / 16], rest[DP / 16];
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            int d = i * 16 + lane / 32 * 8;
+            d = d < a.D ? d : 0;
+            gop[i] = *(const s16x8 *)(grow + d);
+            o[i] = *(const T8 *)((const T *)a.o + at + d);
+            rest[i] = *(const T8 *)((const T *)a.orest + at + d);
+            qop[i] = *(const s16x8 *)(qrow + d);
+        }
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             const int d = i * 16 + lane / 32 * 8;
-            s16x8 x = {}, y = {};
-            if (live && d < a.D) {
-                x = *(const s16x8 *)(qrow + d);
-                y = *(const s16x8 *)(grow + d);
-                float f[8], g[8];
-                ld8<T>(f, out + d);
-                ld8<T>(g, rest + d);
-                const typename vec8<T>::type z =
-                    __builtin_bit_cast(typename vec8<T>::type, y);
+            if (!live || d >= a.D) qop[i] = gop[i] = s16x8{};
+            const T8 z = __builtin_bit_cast(T8, gop[i]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    delta += (f[j] + g[j]) * (float)z[j];
-            }
-            qop[i] = x;
-            gop[i] = y;
+            for (int j = 0; j < 8; ++j)
+                delta += ((float)o[i][j] + (float)rest[i][j]) * (float)z[j];
         }
     }
     delta += other_half(delta);
@@ -817,6 +829,17 @@ __device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
     if (p1 > s.start + a.S - 1) p1 = s.start + a.S - 1;
 }
 
+// Parts of key block k0 that hold anything for the 32 keys from w0: where
+// those are past the first tokens, no more than reach to the end of the
+// last key's window.
+__device__ inline int parts_of(const Args &a, int k0, int w0, int parts)
+{
+    if (k0 >= a.sinks || w0 < a.sinks) return parts;
+    const long long rows = ((long long)k0 + 127 + a.window) * a.G;
+    const long long n = (rows + a.sink_rows - 1) / a.sink_rows;
+    return n < parts ? (int)n : parts;
+}
+
 // What dk and dv need of a tile's rows.
 struct RowData {
     __align__(16) float lse[KT];
@@ -860,20 +883,22 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
 
     s16x8 kop[DP / 16], vop[DP / 16];
     {
-        const short *krow = (const short *)a.k + b * a.kb +
-                            (long long)key * a.ks + h * a.kh;
-        const short *vrow = (const short *)a.v + b * a.vb +
-                            (long long)key * a.vs + h * a.vh;
+        const long long at = key < a.T ? key : a.T - 1;
+        const short *krow =
+            (const short *)a.k + b * a.kb + at * a.ks + h * a.kh;
+        const short *vrow =
+            (const short *)a.v + b * a.vb + at * a.vs + h * a.vh;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            int d = i * 16 + lane / 32 * 8;
+            d = d < a.D ? d : 0;
+            kop[i] = *(const s16x8 *)(krow + d);
+            vop[i] = *(const s16x8 *)(vrow + d);
+        }
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             const int d = i * 16 + lane / 32 * 8;
-            s16x8 x = {}, y = {};
-            if (key < s.n && d < a.D) {
-                x = *(const s16x8 *)(krow + d);
-                y = *(const s16x8 *)(vrow + d);
-            }
-            kop[i] = x;
-            vop[i] = y;
+            if (key >= s.n || d >= a.D) kop[i] = vop[i] = s16x8{};
         }
     }
     int p0, p1;
@@ -1033,7 +1058,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
         t0 += KT;
     }
     if (parts > 1) {
-        if (key >= a.T) return;
+        if (key >= a.T || part >= parts_of(a, k0, w0, parts)) return;
         // parts of a key head: sink blocks', then the others'
         const long long slot =
             blk < a.sink_blocks
@@ -1084,8 +1109,9 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int DP)
     if (key >= a.T) return;
     const int blk = key / 128;
     const bool sink = blk < a.sink_blocks;
-    const int parts = sink ? a.sink_splits : a.splits;
+    int parts = sink ? a.sink_splits : a.splits;
     if (parts == 1) return;  // written where it was summed
+    if (sink) parts = parts_of(a, blk * 128, key & ~31, parts);
     const long long slot =
         sink ? (long long)blk * a.sink_splits
              : (long long)a.sink_blocks * a.sink_splits +
