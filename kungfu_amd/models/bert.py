@@ -4,6 +4,12 @@ benchmark config.
 Self-contained transformer encoder with BERT-base dimensions (L=12, H=768,
 A=12, ~110M params); attention uses torch's fused SDPA, which lowers to the
 ROCm flash-attention path on MI355X.
+
+Options beside the plain encoder, each off by default: `fused_embed` (the
+lookup in the activations' type, gradient by sorted tokens), `qk_norm` and
+`rotary` (norm of queries and keys for each head, positions by rotation
+instead of an embedding), `window`/`sinks`/`causal` (attention to near and
+first tokens), and padded batches by `lengths`.
 """
 import torch
 import torch.nn as nn
@@ -20,10 +26,27 @@ def _make_ln(hidden, fused):
     return nn.LayerNorm(hidden)
 
 
+def _make_embed(n, hidden, fused):
+    if fused:
+        from kungfu_amd.ops.fused_embedding import FusedEmbedding
+
+        return FusedEmbedding(n, hidden)
+    return nn.Embedding(n, hidden)
+
+
 class BertLayer(nn.Module):
-    def __init__(self, hidden, heads, ffn, fused_ln=False):
+    def __init__(self, hidden, heads, ffn, fused_ln=False, qk_norm=False,
+                 window=None, sinks=0, causal=False):
         super().__init__()
         self.heads = heads
+        self.window = window
+        self.sinks = sinks
+        self.causal = causal
+        self.qk = None
+        if qk_norm:
+            from kungfu_amd.ops.qk_norm_rope import QKNormRope
+
+            self.qk = QKNormRope(hidden // heads)
         # KfLinear = nn.Linear + fused column-sum bias-grad kernel
         # (native autograd fallback outside the bf16-master conditions)
         self.qkv = KfLinear(hidden, 3 * hidden)
@@ -33,12 +56,25 @@ class BertLayer(nn.Module):
         self.fc2 = KfLinear(ffn, hidden)
         self.ln2 = _make_ln(hidden, fused_ln)
 
-    def forward(self, x):
+    def attend(self, qkv, rope, lengths):
+        if self.qk is None and rope is None and self.window is None and \
+                not self.causal and lengths is None:
+            q, k, v = (t.transpose(1, 2) for t in qkv.unbind(2))
+            a = F.scaled_dot_product_attention(q, k, v)
+            return a.transpose(1, 2)
+        from kungfu_amd.ops.window_attention import window_attention
+
+        q, k, v = qkv.unbind(2)
+        if self.qk is not None:
+            q, k = self.qk(q, k, rope)
+        return window_attention(q, k, v, window=self.window,
+                                sinks=self.sinks, causal=self.causal,
+                                lengths=lengths)
+
+    def forward(self, x, rope=None, lengths=None):
         b, s, h = x.shape
         qkv = self.qkv(x).view(b, s, 3, self.heads, h // self.heads)
-        q, k, v = (t.transpose(1, 2) for t in qkv.unbind(2))
-        a = F.scaled_dot_product_attention(q, k, v)
-        a = a.transpose(1, 2).reshape(b, s, h)
+        a = self.attend(qkv, rope, lengths).reshape(b, s, h)
         x = self.ln1(x + self.proj(a))
         x = self.ln2(x + self.fc2(F.gelu(self.fc1(x))))
         return x
@@ -46,14 +82,25 @@ class BertLayer(nn.Module):
 
 class Bert(nn.Module):
     def __init__(self, vocab=30522, hidden=768, layers=12, heads=12,
-                 ffn=3072, max_len=512, fused_ln=False):
+                 ffn=3072, max_len=512, fused_ln=False, fused_embed=False,
+                 qk_norm=False, rotary=False, window=None, sinks=0,
+                 causal=False):
         super().__init__()
+        if rotary and not qk_norm:
+            raise ValueError("rotary positions need qk_norm")
         self.fused_ln = fused_ln
-        self.tok = nn.Embedding(vocab, hidden)
-        self.pos = nn.Embedding(max_len, hidden)
+        self.fused_embed = fused_embed
+        self.tok = _make_embed(vocab, hidden, fused_embed)
+        self.pos = None
+        if not rotary:
+            self.pos = _make_embed(max_len, hidden, fused_embed)
+        self.rotary = (max_len, hidden // heads) if rotary else None
+        self._rope = None
         self.ln = _make_ln(hidden, fused_ln)
         self.blocks = nn.ModuleList(
-            [BertLayer(hidden, heads, ffn, fused_ln=fused_ln)
+            [BertLayer(hidden, heads, ffn, fused_ln=fused_ln,
+                       qk_norm=qk_norm, window=window, sinks=sinks,
+                       causal=causal)
              for _ in range(layers)])
         self.head = KfLinear(hidden, vocab)
         for m in self.modules():
@@ -63,17 +110,45 @@ class Bert(nn.Module):
             elif isinstance(m, nn.Embedding):
                 nn.init.normal_(m.weight, std=0.02)
 
-    def forward(self, ids):
-        b, s = ids.shape
-        pos = torch.arange(s, device=ids.device).unsqueeze(0)
-        x = self.tok(ids) + self.pos(pos)
-        if self.fused_ln and x.is_cuda:
+    def _lookup(self, table, ids, low):
+        if not self.fused_embed:
+            return table(ids)
+        from kungfu_amd.ops.fused_embedding import embedding
+
+        # in the activations' type: no cast of the rows after it
+        return embedding(ids, table.weight,
+                         out_dtype=torch.bfloat16 if low else None)
+
+    def _embed(self, ids):
+        low = self.fused_ln and ids.is_cuda
+        x = self._lookup(self.tok, ids, low)
+        if self.pos is not None:
+            pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
+            x = x + self._lookup(self.pos, pos, low)
+        if low:
             x = x.to(torch.bfloat16)  # embeddings stay fp32 under autocast
-        x = self.ln(x)
+        return self.ln(x)
+
+    def _angles(self, device):
+        # no buffer: the table stays f32 when the model's type is changed
+        if self.rotary is None:
+            return None
+        if self._rope is None or self._rope.device != device:
+            from kungfu_amd.ops.qk_norm_rope import rope_table
+
+            self._rope = rope_table(*self.rotary, device=device)
+        return self._rope
+
+    def forward(self, ids, lengths=None):
+        """Logits of every token. `lengths` (batch,) are the tokens that
+        each sequence of a padded batch has: no token attends to what lies
+        behind them."""
+        x = self._embed(ids)
+        rope = self._angles(ids.device)
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x, rope, lengths)
         return self.head(x)
 
 
-def bert_base(vocab=30522, max_len=512, fused_ln=False):
-    return Bert(vocab=vocab, max_len=max_len, fused_ln=fused_ln)
+def bert_base(vocab=30522, max_len=512, fused_ln=False, **options):
+    return Bert(vocab=vocab, max_len=max_len, fused_ln=fused_ln, **options)
