@@ -376,19 +376,14 @@ struct Cols {
 };
 
 template <typename T, int PER>
-__device__ inline void load_n(float *f, const T *p)
-{
-    constexpr int A = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
-    typedef __attribute__((ext_vector_type(PER), aligned(A))) T V;
-    const V v = *(const V *)p;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) f[i] = (float)v[i];
-}
+struct Piece {
+    static constexpr int A = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
+    typedef __attribute__((ext_vector_type(PER), aligned(A))) T type;
+};
 template <typename T, int PER>
 __device__ inline void store_n(T *p, const float *f)
 {
-    constexpr int A = PER * sizeof(T) < 16 ? PER * sizeof(T) : 16;
-    typedef __attribute__((ext_vector_type(PER), aligned(A))) T V;
+    typedef typename Piece<T, PER>::type V;
     V v;
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = (T)f[i];
@@ -401,7 +396,8 @@ template <typename T, typename C, int U, typename Idx>
 __device__ inline void add_rows(float *acc, const T *base, int n, int c0,
                                 int lane, int H, Idx idx)
 {
-    float f[U][8];
+    typedef typename Piece<T, C::PER>::type V;
+    V f[U][C::GROUPS];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const T *row = base + (long long)idx(u < n ? u : 0) * H;
@@ -410,15 +406,15 @@ __device__ inline void add_rows(float *acc, const T *base, int n, int c0,
             // a branch around a load would wait for it; lanes past the
             // last column repeat it, and their sums are not stored
             const int c = C::at(c0, lane, g);
-            load_n<T, C::PER>(&f[u][g * C::PER],
-                              row + (c < H ? c : H - C::PER));
+            f[u][g] = *(const V *)(row + (c < H ? c : H - C::PER));
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (u < n)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += f[u][j];
+            for (int j = 0; j < 8; ++j)
+                acc[j] += (float)f[u][j / C::PER][j % C::PER];
 }
 
 // Sums of CHUNK neighbours of the sorted order that belong to one token,
@@ -484,6 +480,8 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
     int H, int slices, float scale)
 {
     typedef Cols<W, VEC> C;
+    // rows on their way at once: 32 registers of them
+    constexpr int U = sizeof(T) == 2 ? 8 : 4;
     const int lane = threadIdx.x % WAVE;
     for (long long u = (long long)blockIdx.x * WAVES + threadIdx.x / WAVE;
          u < units; u += (long long)gridDim.x * WAVES) {
@@ -500,11 +498,11 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
                 // up to the next chunk, or to the end
                 const int here = CHUNK - i % CHUNK;
                 int n = here < left ? here : left;
-                n = n < 8 ? n : 8;
+                n = n < U ? n : U;
                 // no more loads than twice the rows that are there
                 auto row = [&](int k) { return pos[i + k]; };
                 if (n > 4)
-                    add_rows<T, C, 8>(acc, dout, n, c0, lane, H, row);
+                    add_rows<T, C, U>(acc, dout, n, c0, lane, H, row);
                 else if (n > 2)
                     add_rows<T, C, 4>(acc, dout, n, c0, lane, H, row);
                 else if (n > 1)
@@ -517,15 +515,15 @@ __global__ __launch_bounds__(BLOCK) void embed_rows(
                 int n = left / CHUNK;
                 const int here = (BIG - i % BIG) / CHUNK;
                 n = part2 && here < n ? here : n;
-                n = n < 8 ? n : 8;
-                add_rows<float, C, 8>(acc, part1, n, c0, lane, H, [&](int k) {
+                n = n < 4 ? n : 4;
+                add_rows<float, C, 4>(acc, part1, n, c0, lane, H, [&](int k) {
                     return i / CHUNK + k;
                 });
                 i += n * CHUNK;
             } else {
                 int n = left / BIG;
-                n = n < 8 ? n : 8;
-                add_rows<float, C, 8>(acc, part2, n, c0, lane, H,
+                n = n < 4 ? n : 4;
+                add_rows<float, C, 4>(acc, part2, n, c0, lane, H,
                                       [&](int k) { return i / BIG + k; });
                 i += n * BIG;
             }

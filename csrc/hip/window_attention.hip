@@ -634,43 +634,64 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         a.lse[row] = l == 0.f ? __builtin_inff() : m * a.c + log2f(l);
 }
 
-// Joins the parts of a row: one wave a row, DP / 64 columns a lane.
+// Joins the parts of a row, one block a row: each wave a quarter of them
+// in order, against the quarter's own maximum, then the quarters in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 {
-    const int lane = threadIdx.x % WAVE;
-    const int SG = a.S * a.G;
-    const long long row = (long long)blockIdx.x * 4 + threadIdx.x / WAVE;
-    if (row >= (long long)a.B * a.Hk * SG) return;
+    __shared__ float mq[4], lq[4], oq[4][128];
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    const long long row = blockIdx.x;
     const float *ml = a.part_ml + row * a.splits * 2;
+    const int p0 = (int)((long long)a.splits * wid / 4);
+    const int p1 = (int)((long long)a.splits * (wid + 1) / 4);
     float m = -__builtin_inff();
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[2 * i]);
-    const float base = m == -__builtin_inff() ? 0.f : m;
+    for (int i = p0 + lane; i < p1; i += WAVE) m = fmaxf(m, ml[2 * i]);
+    for (int off = WAVE / 2; off > 0; off >>= 1)
+        m = fmaxf(m, __shfl_xor(m, off));
+    float base = m == -__builtin_inff() ? 0.f : m;
     float l = 0.f, o[2] = {};
-    for (int i = 0; i < a.splits; ++i) {
+    // columns past DP repeat the last one and are not written
+    const int c0 = lane < DP ? lane : DP - 1;
+    const int c1 = lane + 64 < DP ? lane + 64 : DP - 1;
+    const float *po = a.part_o + row * a.splits * DP;
+#pragma unroll 8
+    for (int i = p0; i < p1; ++i) {
         const float w = __builtin_amdgcn_exp2f(ml[2 * i] - base);
         l += w * ml[2 * i + 1];
-        const float *po = a.part_o + (row * a.splits + i) * DP;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (lane + j * 64 < a.D) o[j] += w * po[lane + j * 64];
+        o[0] += w * po[(long long)i * DP + c0];
+        o[1] += w * po[(long long)i * DP + c1];
     }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    const long long bh = row / SG;
-    const int r = (int)(row - bh * SG), qi = r / a.G, g = r - qi * a.G;
-    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
-    T *out = (T *)a.out +
-             (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D;
+    if (lane == 0) {
+        mq[wid] = m;
+        lq[wid] = l;
+    }
+    oq[wid][lane] = o[0];
+    oq[wid][lane + 64] = o[1];
+    __syncthreads();
+    m = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+    base = m == -__builtin_inff() ? 0.f : m;
+    const int c = threadIdx.x % 128;
+    float x = 0.f;
+    l = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (lane + j * 64 < a.D) {
-            const float f = o[j] * inv;
-            out[lane + j * 64] = (T)f;
-            if (a.rest)
-                ((T *)a.rest)[out - (T *)a.out + lane + j * 64] =
-                    (T)(f - (float)(T)f);
-        }
-    if (a.lse && lane == 0)
+    for (int i = 0; i < 4; ++i) {
+        const float w = __builtin_amdgcn_exp2f(mq[i] - base);
+        l += w * lq[i];
+        x += w * oq[i][c];
+    }
+    const float f = l > 0.f ? x / l : l == 0.f ? 0.f : l;
+    const long long bh = row / (a.S * a.G);
+    const int r = (int)(row - bh * (a.S * a.G)), qi = r / a.G;
+    const int g = r - qi * a.G;
+    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
+    const long long at =
+        (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D + c;
+    if (threadIdx.x < 128 && c < a.D) {
+        ((T *)a.out)[at] = (T)f;
+        if (a.rest) ((T *)a.rest)[at] = (T)(f - (float)(T)f);
+    }
+    if (a.lse && threadIdx.x == 0)
         a.lse[row] = l == 0.f ? __builtin_inff() : base + log2f(l);
 }
 
@@ -1259,9 +1280,9 @@ hipError_t launch_fwd(Args &a, const FwdPlan &p, hipStream_t s)
         else
             attn_fwd<T, DP, 4, false><<<grid, 256, 0, s>>>(a);
     }
-    if (p.splits > 1) {
+    if (p.splits > 1) {  // rows of few blocks, so few
         const long long rows = (long long)a.B * a.Hk * a.S * a.G;
-        attn_join<T><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a, DP);
+        attn_join<T><<<(unsigned)rows, 256, 0, s>>>(a, DP);
     }
     return hipGetLastError();
 }

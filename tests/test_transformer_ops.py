@@ -632,6 +632,75 @@ def test_attention_of_nothing(device):
     assert not dq.any()
 
 
+# ---- offsets past 32 bits ----
+
+@gpu
+def test_embedding_of_a_table_past_32_bits():
+    """Rows whose first element is past 2^31."""
+    V, H = (1 << 21) + 77, 1024
+    w = torch.zeros(V, H, dtype=BF16, device="cuda")
+    ids = torch.tensor([V - 1, 5, 1 << 21, V - 1], device="cuda")
+    gen = torch.Generator().manual_seed(18)
+    rows = randn(gen, (3, H), BF16, "cuda")
+    for i, n in enumerate((V - 1, 5, 1 << 21)):
+        w[n] = rows[i]
+    w.requires_grad_(True)
+    out = embedding(ids, w)
+    assert torch.equal(out, rows[[0, 1, 2, 0]])
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    for n, k in ((V - 1, 2), (5, 1), (1 << 21, 1)):
+        assert (dw[n] == k).all()
+    assert float(dw.sum(dtype=torch.float32)) == 4 * H
+
+
+@gpu
+def test_norm_rope_of_rows_past_32_bits():
+    S, Hq, D = 140011, 120, 128
+    gen = torch.Generator().manual_seed(19)
+    q = torch.zeros(1, S, Hq, D, dtype=BF16, device="cuda")
+    k = torch.zeros(1, S, 1, D, dtype=BF16, device="cuda")
+    at = [0, S // 2, S - 1]
+    for n in at:
+        q[:, n] = randn(gen, (1, Hq, D), BF16, "cuda")
+    rope = rope_table(S, D, device="cuda")
+    q.requires_grad_(True)
+    y, _ = qk_norm_rope(q, k, rope=rope)
+    dq, = torch.autograd.grad(y, q, torch.ones_like(y))
+    for n in at:
+        few = q.detach()[:, n:n + 1].clone().requires_grad_(True)
+        z, _ = qk_norm_rope(few, few[:, :, :1].detach(), rope=rope, start=n)
+        assert torch.equal(z, y[:, n:n + 1])
+        dz, = torch.autograd.grad(z, few, torch.ones_like(z))
+        assert torch.equal(dz, dq[:, n:n + 1])
+
+
+@gpu
+def test_attention_of_a_cache_past_32_bits():
+    """A long cache of which the window and the first tokens are seen."""
+    T, H, D = (1 << 21) + 1003, 8, 128
+    gen = torch.Generator().manual_seed(20)
+    k = torch.full((1, T, H, D), 0.5, dtype=BF16, device="cuda")
+    v = torch.full((1, T, H, D), -2.0, dtype=BF16, device="cuda")
+    seen = list(range(3)) + list(range(T - 80, T))
+    for t in (k, v):
+        t[:, seen] = randn(gen, (1, len(seen), H, D), BF16, "cuda")
+    q = randn(gen, (1, 2, 16, D), BF16, "cuda")
+    dout = randn(gen, q.shape, BF16, "cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*leaves, window=79, sinks=3)
+    grads = torch.autograd.grad(out, leaves, dout)
+    # the same rows and keys alone
+    few = [q.detach().clone().requires_grad_(True)] + [
+        t.detach()[:, seen].clone().requires_grad_(True) for t in (k, v)]
+    want, bound = attn_oracle(*few, dout, 79, 3, True, None, None,
+                              D ** -0.5)
+    inside(out, want["out"], bound["out"], "out")
+    inside(grads[0], want["dq"], bound["dq"], "dq")
+    for i, n in ((1, "dk"), (2, "dv")):
+        inside(grads[i][:, seen], want[n], bound[n], n)
+        assert not grads[i][:, 3:T - 80].any()
+
+
 # ---- together -------------------------------------------------------------
 
 def block(ids, table, qw, kw, proj, rope, heads, lengths=None):
