@@ -13,6 +13,8 @@
 #include <string>
 #include <vector>
 
+#include "kernel_api.h"
+
 namespace py = pybind11;
 
 extern "C" {
@@ -78,17 +80,39 @@ void check(hipError_t e, const char *what)
     }
 }
 
-// Lists cross from Python as vectors; the kernels' entries read a fixed
-// number of each.
-template <typename T>
-const T *list(const std::vector<T> &v, size_t n, const char *what)
-{
-    if (v.size() != n)
-        throw std::invalid_argument(std::string(what) + ": wrong list");
-    return v.data();
-}
-typedef std::vector<uintptr_t> Ptrs;
-typedef std::vector<long long> Dims;
+kf_kernels kernels = {
+    [](int e) { return hipGetErrorString((hipError_t)e); },
+    [](long long N, long long V, int H) {
+        return (long long)kf_embed_ws(N, V, H);
+    },
+    [](const void *ids, int wide, const void *w, long long ldw, int wtype,
+       void *out, int otype, long long N, long long V, int H, float scale,
+       void *stream) {
+        return (int)kf_embed_fwd(ids, wide, w, ldw, wtype, out, otype, N, V,
+                                 H, scale, stream);
+    },
+    [](const void *ids, int wide, const void *dout, int otype, void *dw,
+       int wtype, long long N, long long V, int H, long long padding,
+       float scale, void *work, void *stream) {
+        return (int)kf_embed_bwd(ids, wide, dout, otype, dw, wtype, N, V, H,
+                                 padding, scale, work, stream);
+    },
+    kf_qk_ws,
+    [](const uintptr_t *ptrs, const long long *dims, int dtype, float eps,
+       int backward, void *stream) {
+        return (int)kf_qk_norm_rope(ptrs, dims, dtype, eps, backward,
+                                    stream);
+    },
+    kf_attn_ws,
+    [](const uintptr_t *ptrs, const long long *dims,
+       const long long *strides, float scale, int dtype, void *stream) {
+        return (int)kf_attn_fwd(ptrs, dims, strides, scale, dtype, stream);
+    },
+    [](const uintptr_t *ptrs, const long long *dims,
+       const long long *strides, float scale, int dtype, void *stream) {
+        return (int)kf_attn_bwd(ptrs, dims, strides, scale, dtype, stream);
+    },
+};
 
 struct ChunkHost {
     const void *src;
@@ -300,65 +324,8 @@ PYBIND11_MODULE(_hip, m)
         check(kf_ln_fold((void *)wb, H, (void *)stream), "kf_ln_fold");
     });
 
-    // ---- embedding lookup with a scale, gradient by sorted tokens ----
-    m.def("embed_ws", [](long long N, long long V, int H) {
-        return (long long)kf_embed_ws(N, V, H);
-    });
-    m.def("embed_fwd",
-          [](uintptr_t ids, bool wide, uintptr_t w, long long ldw, int wtype,
-             uintptr_t out, int otype, long long N, long long V, int H,
-             float scale, uintptr_t stream) {
-              check(kf_embed_fwd((const void *)ids, wide ? 1 : 0,
-                                 (const void *)w, ldw, wtype, (void *)out,
-                                 otype, N, V, H, scale, (void *)stream),
-                    "kf_embed_fwd");
-          });
-    m.def("embed_bwd",
-          [](uintptr_t ids, bool wide, uintptr_t dout, int otype,
-             uintptr_t dw, int wtype, long long N, long long V, int H,
-             long long padding, float scale, uintptr_t work,
-             uintptr_t stream) {
-              check(kf_embed_bwd((const void *)ids, wide ? 1 : 0,
-                                 (const void *)dout, otype, (void *)dw,
-                                 wtype, N, V, H, padding, scale,
-                                 (void *)work, (void *)stream),
-                    "kf_embed_bwd");
-          });
-
-    // ---- query/key norm for each head with the position rotation ----
-    m.def("qk_ws", [](int D, int heads) { return kf_qk_ws(D, heads); });
-    m.def("qk_norm_rope",
-          [](const Ptrs &ptrs, const Dims &dims, int dtype, float eps,
-             bool backward, uintptr_t stream) {
-              check(kf_qk_norm_rope(
-                        list(ptrs, backward ? 13 : 8, "qk_norm_rope"),
-                        list(dims, backward ? 23 : 17, "qk_norm_rope"),
-                        dtype, eps, backward ? 1 : 0, (void *)stream),
-                    "kf_qk_norm_rope");
-          });
-
-    // ---- attention with a sliding window and first tokens ----
-    m.def("attn_ws", [](const Dims &dims, bool backward) {
-        return kf_attn_ws(list(dims, 9, "attn_ws"), backward ? 1 : 0);
-    });
-    m.def("attn_fwd",
-          [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
-             float scale, int dtype, uintptr_t stream) {
-              check(kf_attn_fwd(list(ptrs, 9, "attn_fwd"),
-                                list(dims, 9, "attn_fwd"),
-                                list(strides, 9, "attn_fwd"), scale, dtype,
-                                (void *)stream),
-                    "kf_attn_fwd");
-          });
-    m.def("attn_bwd",
-          [](const Ptrs &ptrs, const Dims &dims, const Dims &strides,
-             float scale, int dtype, uintptr_t stream) {
-              check(kf_attn_bwd(list(ptrs, 13, "attn_bwd"),
-                                list(dims, 9, "attn_bwd"),
-                                list(strides, 12, "attn_bwd"), scale, dtype,
-                                (void *)stream),
-                    "kf_attn_bwd");
-          });
+    // ---- the transformer kernels, for the autograd nodes of `_nodes` ----
+    m.attr("kernels") = py::capsule(&kernels, KF_KERNELS_CAPSULE);
 
     // ---- fused BatchNorm(+residual+ReLU), NHWC bf16 ----
     m.def("bn_stats",

@@ -10,10 +10,8 @@ cast of the gradient where the activations are of another type.
 On CPU tensors the same is computed by eager torch.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from kungfu_amd.ops import hip
-from kungfu_amd.utils.dtypes import hip_dtype
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -47,48 +45,6 @@ def _check(ids, weight, padding_idx, out_dtype):
                          "a width of 2^20")
 
 
-def _forward(ids, weight, scale, out_dtype):
-    h = hip._require()
-    w = weight if weight.stride(1) == 1 or weight.shape[1] == 1 else \
-        weight.contiguous()
-    out = weight.new_empty(ids.shape + weight.shape[1:], dtype=out_dtype)
-    if ids.numel():
-        with hip.on_device(weight):
-            h.embed_fwd(ids.data_ptr(), ids.dtype == torch.int64,
-                        w.data_ptr(), w.stride(0), hip_dtype(w.dtype),
-                        out.data_ptr(), hip_dtype(out_dtype), ids.numel(),
-                        w.shape[0], w.shape[1], scale, hip.stream_of(w))
-    return out
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx, out_dtype):
-        ctx.save_for_backward(ids)
-        ctx.of = (weight.shape, weight.dtype, scale, padding_idx, out_dtype)
-        return _forward(ids, weight, scale, out_dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        ids, = ctx.saved_tensors
-        (V, H), dtype, scale, padding_idx, out_dtype = ctx.of
-        h = hip._require()
-        if dout.dtype != out_dtype:
-            dout = dout.to(out_dtype)
-        dout = dout.contiguous()
-        dw = dout.new_empty((V, H), dtype=dtype)
-        N = ids.numel()
-        with hip.on_device(dout):
-            ws = dout.new_empty(h.embed_ws(N, V, H), dtype=torch.uint8)
-            h.embed_bwd(ids.data_ptr(), ids.dtype == torch.int64,
-                        dout.data_ptr(), hip_dtype(out_dtype), dw.data_ptr(),
-                        hip_dtype(dtype), N, V, H,
-                        -1 if padding_idx is None else padding_idx, scale,
-                        ws.data_ptr(), hip.stream_of(dout))
-        return None, dw, None, None, None
-
-
 def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     """scale * weight[ids], as `out_dtype` (default: the weight's type).
 
@@ -109,10 +65,12 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
         if weight.dtype != torch.float64:
             rows = rows.float()
         return (rows * scale).to(out_dtype)
-    ids = ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(ids, weight, scale, padding_idx, out_dtype)
-    return _forward(ids, weight, scale, out_dtype)
+    if weight.stride(1) != 1 and weight.shape[1] > 1:
+        weight = weight.contiguous()
+    return hip.nodes().embedding(
+        ids.contiguous(), weight, scale,
+        -1 if padding_idx is None else padding_idx, out_dtype,
+        hip.stream_of(weight))
 
 
 class FusedEmbedding(torch.nn.Embedding):

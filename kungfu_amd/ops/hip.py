@@ -11,6 +11,10 @@ try:
     from kungfu_amd import _hip
 except ImportError:  # pragma: no cover - CPU-only environments
     _hip = None
+try:
+    from kungfu_amd import _nodes
+except ImportError:  # pragma: no cover - CPU-only environments
+    _nodes = None
 
 from kungfu_amd.utils.dtypes import hip_dtype
 
@@ -214,37 +218,25 @@ def transform2(z, x, op="sum"):
 
 # ---- what the transformer ops share ----
 
-class _Here:
-    def __enter__(self):
-        pass
+def nodes():
+    """The transformer ops' autograd nodes (csrc/torch/nodes.cpp)."""
+    if _nodes is None:
+        _require()
+        raise RuntimeError(
+            "kungfu_amd._nodes is not built; run `python setup.py build_ext "
+            "--inplace` (it is mandatory on GPU hosts)")
+    return _nodes
 
-    def __exit__(self, *exc):
-        pass
 
-
-_HERE = _Here()
-# The current device and its stream as numbers, without the Python objects
-# around them, which cost as much as a small kernel.
-_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+# The current stream's handle as a number, without the Python object around
+# it, which costs as much as a small kernel.
 _stream_now = getattr(
     torch._C, "_cuda_getCurrentRawStream",
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def on_device(t):
-    """Makes t's device current, for a launch on its stream."""
-    index = t.get_device()
-    return _HERE if _device_now() == index else torch.cuda.device(index)
-
-
 def stream_of(t):
     return _stream_now(t.get_device())
-
-
-def dense_like(t):
-    """An uninitialised tensor of t's shape and type, row-major whatever
-    t's strides are."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def row_strides(t):

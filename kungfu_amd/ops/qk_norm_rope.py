@@ -9,10 +9,8 @@ them.
 On CPU tensors the same is computed by eager torch.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from kungfu_amd.ops import hip
-from kungfu_amd.utils.dtypes import hip_dtype
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -101,69 +99,6 @@ def _dense_rows(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _launch(q, k, qw, kw, oq, ok, rope, positions, start, eps, grads=None):
-    B, S, Hq, D = q.shape
-    pb = ps = 0
-    if positions is not None:
-        ps = positions.stride(-1)
-        pb = positions.stride(0) if positions.dim() == 2 else 0
-    w = qw if qw is not None else kw
-    ptrs = [q.data_ptr(), k.data_ptr(), _ptr(qw), _ptr(kw), oq.data_ptr(),
-            ok.data_ptr(), _ptr(rope), _ptr(positions)]
-    dims = [B * S, S, D, Hq, k.shape[2], *hip.row_strides(q),
-            *hip.row_strides(k), 0 if rope is None else rope.shape[0],
-            start, pb, ps,
-            positions is not None and positions.dtype == torch.int64,
-            w is not None and w.dtype == torch.float32]
-    if grads is not None:
-        dyq, dyk, dqw, dkw, partial = grads
-        ptrs += [dyq.data_ptr(), dyk.data_ptr(), _ptr(dqw), _ptr(dkw),
-                 _ptr(partial)]
-        dims += [*hip.row_strides(dyq), *hip.row_strides(dyk)]
-    hip._require().qk_norm_rope(ptrs, dims, hip_dtype(q.dtype), eps,
-                                grads is not None, hip.stream_of(q))
-
-
-def _forward(q, k, qw, kw, rope, positions, start, eps):
-    oq, ok = hip.dense_like(q), hip.dense_like(k)
-    if oq.numel() or ok.numel():
-        with hip.on_device(q):
-            _launch(q, k, qw, kw, oq, ok, rope, positions, start, eps)
-    return oq, ok
-
-
-class _QKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, qw, kw, rope, positions, start, eps):
-        ctx.save_for_backward(q, k, qw, kw, rope, positions)
-        ctx.of = (start, eps)
-        return _forward(q, k, qw, kw, rope, positions, start, eps)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dyq, dyk):
-        q, k, qw, kw, rope, positions = ctx.saved_tensors
-        start, eps = ctx.of
-        dyq, dyk = _dense_rows(dyq), _dense_rows(dyk)
-        dq, dk = hip.dense_like(q), hip.dense_like(k)
-        dqw = None if qw is None else torch.empty_like(qw)
-        dkw = None if kw is None else torch.empty_like(kw)
-        partial = None
-        if q.shape[2] + k.shape[2]:
-            with hip.on_device(q):
-                if dqw is not None or dkw is not None:
-                    size = hip._require().qk_ws(
-                        q.shape[3], q.shape[2] + k.shape[2])
-                    partial = q.new_empty(size, dtype=torch.float32)
-                _launch(q, k, qw, kw, dq, dk, rope, positions, start, eps,
-                        (dyq, dyk, dqw, dkw, partial))
-        return dq, dk, dqw, dkw, None, None, None, None
-
-
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, rope=None,
                  positions=None, start=0, eps=1e-6):
     """Norms and rotates q (batch, length, heads, width) and k (batch,
@@ -192,12 +127,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, rope=None,
         q_weight = q_weight.contiguous()
     if k_weight is not None:
         k_weight = k_weight.contiguous()
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad
-            for t in (q, k, q_weight, k_weight)):
-        return _QKNormRope.apply(q, k, q_weight, k_weight, rope, positions,
-                                 start, eps)
-    return _forward(q, k, q_weight, k_weight, rope, positions, start, eps)
+    return hip.nodes().qk_norm_rope(q, k, q_weight, k_weight, rope,
+                                    positions, start, eps, hip.stream_of(q))
 
 
 class QKNormRope(torch.nn.Module):

@@ -11,10 +11,8 @@ On CPU tensors the same is computed by eager torch.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from kungfu_amd.ops import hip
-from kungfu_amd.utils.dtypes import hip_dtype
 
 _MOST = 1 << 30
 
@@ -96,73 +94,11 @@ def _eager(q, k, v, window, sinks, causal, lengths, starts, scale):
     return out.reshape(B, Hq, S, D).transpose(1, 2)
 
 
-def _dims(q, k, window, sinks, causal):
-    return [q.shape[0], q.shape[1], k.shape[1], k.shape[2],
-            q.shape[2] // k.shape[2], q.shape[3],
-            _MOST if window is None else min(window, _MOST),
-            min(sinks, _MOST), causal]
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
 def _int32(t):
     """Positions as the kernels read them; far ones stay far."""
     if t.dtype == torch.int64:
         t = t.clamp(-_MOST, _MOST).to(torch.int32)
     return t.contiguous()
-
-
-def _forward(q, k, v, dims, lengths, starts, scale, keep):
-    """The output and, to keep for the backward, each row's log-sum-exp in
-    powers of two and what rounding took off the output."""
-    h = hip._require()
-    out = hip.dense_like(q)
-    lse = rest = None
-    if keep:
-        lse = q.new_empty(dims[0] * dims[1] * q.shape[2],
-                          dtype=torch.float32)
-        rest = hip.dense_like(q)
-    strides = [*hip.row_strides(q), *hip.row_strides(k),
-               *hip.row_strides(v)]
-    with hip.on_device(q):
-        size = h.attn_ws(dims, False)
-        ws = q.new_empty(size, dtype=torch.uint8) if size > 0 else None
-        h.attn_fwd([q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                    out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(lengths),
-                    _ptr(starts), _ptr(ws)], dims, strides, scale,
-                   hip_dtype(q.dtype), hip.stream_of(q))
-    return out, lse, rest, strides
-
-
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, dims, lengths, starts, scale):
-        out, lse, rest, strides = _forward(q, k, v, dims, lengths, starts,
-                                           scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, rest, lengths, starts)
-        ctx.of = (dims, scale, strides)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, rest, lengths, starts = ctx.saved_tensors
-        dims, scale, strides = ctx.of
-        h = hip._require()
-        dout = hip.rows16(dout)
-        dq, dk, dv = hip.dense_like(q), hip.dense_like(k), hip.dense_like(v)
-        with hip.on_device(q):
-            ws = q.new_empty(h.attn_ws(dims, True), dtype=torch.uint8)
-            h.attn_bwd([q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                        out.data_ptr(), lse.data_ptr(), rest.data_ptr(),
-                        _ptr(lengths), _ptr(starts), dout.data_ptr(),
-                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                        ws.data_ptr()], dims,
-                       strides + hip.row_strides(dout), scale,
-                       hip_dtype(q.dtype), hip.stream_of(q))
-        return dq, dk, dv, None, None, None, None
 
 
 def window_attention(q, k, v, window=None, sinks=0, causal=True,
@@ -201,13 +137,12 @@ def window_attention(q, k, v, window=None, sinks=0, causal=True,
         every = torch.ones((), dtype=torch.bool, device=q.device)
         q, k, v = (t.masked_fill(every, 0) for t in (q, k, v))
         return q + k.sum() + v.sum()
-    dims = _dims(q, k, window, sinks, bool(causal))
     q, k, v = hip.rows16(q), hip.rows16(k), hip.rows16(v)
     if lengths is not None:
         lengths = _int32(lengths)
     if starts is not None:
         starts = _int32(starts)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
-                                    v.requires_grad):
-        return _WindowAttention.apply(q, k, v, dims, lengths, starts, scale)
-    return _forward(q, k, v, dims, lengths, starts, scale, False)[0]
+    return hip.nodes().window_attention(
+        q, k, v, lengths, starts, _MOST if window is None else
+        min(window, _MOST), min(sinks, _MOST), bool(causal), scale,
+        hip.stream_of(q))

@@ -1,11 +1,15 @@
 """Build the KungFu-AMD native extensions in-tree.
 
-Two extensions:
+Extensions:
   kungfu_amd._core — C++17 control plane + CPU collective engine (g++).
   kungfu_amd._hip  — hand-written gfx950 HIP kernels (hipcc, pybind11 host
                      bindings; tensors are passed as raw device pointers and
                      HIP streams as integers, so no torch headers and no
                      hipify are involved).
+  kungfu_amd._rccl — native RCCL layer (hipcc).
+  kungfu_amd._nodes — autograd nodes of the transformer operators (g++ with
+                     torch's headers; the kernels come from _hip in a
+                     capsule, so no HIP headers are involved).
 
 Usage: python setup.py build_ext --inplace
 """
@@ -101,6 +105,34 @@ def build_rccl_ext(out_dir):
                                   "-Wl,-rpath,/opt/rocm/lib"])
 
 
+def build_nodes_ext(out_dir):
+    """The autograd nodes, against the installed torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = os.path.join(ROOT, "csrc", "torch", "nodes.cpp")
+    out = os.path.join(out_dir,
+                       "_nodes" + sysconfig.get_config_var("EXT_SUFFIX"))
+    deps = [src, os.path.join(ROOT, "csrc", "hip", "kernel_api.h"),
+            os.path.abspath(__file__)]
+    if os.path.exists(out) and \
+            os.path.getmtime(out) > max(map(os.path.getmtime, deps)):
+        return out
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-O2",
+           "-std=c++17", src, "-o", out,
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(),
+           "-I" + sysconfig.get_paths()["include"]]
+    cmd += ["-isystem" + d for d in cpp_extension.include_paths()]
+    cmd += ["-L" + lib, "-Wl,-rpath," + lib, "-ltorch_python", "-ltorch",
+            "-ltorch_cpu", "-lc10"]
+    print("+", " ".join(cmd))
+    subprocess.check_call(cmd)
+    return out
+
+
 class BuildExt(build_ext):
     def run(self):
         super().run()
@@ -109,8 +141,10 @@ class BuildExt(build_ext):
                 dest = os.path.join(ROOT, "kungfu_amd")
                 build_hip_ext(dest)
                 build_rccl_ext(dest)
+                build_nodes_ext(dest)
             else:
-                print("hipcc not found; skipping kungfu_amd._hip/_rccl")
+                print("hipcc not found; skipping kungfu_amd._hip/_rccl/"
+                      "_nodes")
 
 
 core_ext = Extension(

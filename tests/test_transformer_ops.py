@@ -632,6 +632,43 @@ def test_attention_of_nothing(device):
     assert not dq.any()
 
 
+@gpu
+def test_no_second_derivative():
+    """A second differentiation is refused, not zero."""
+    w = torch.randn(9, 16, device="cuda", requires_grad=True)
+    ids = torch.arange(5, device="cuda")
+    q = torch.randn(1, 4, 2, 32, device="cuda", requires_grad=True)
+    a = torch.randn(1, 4, 2, 32, device="cuda").bfloat16()
+    a.requires_grad_(True)
+    for x, y in ((w, embedding(ids, w)), (q, qk_norm_rope(q, q)[0]),
+                 (a, window_attention(a, a, a))):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        assert torch.isfinite(g).all()
+        with pytest.raises(RuntimeError, match="second derivative"):
+            g.sum().backward()
+
+
+@gpu
+def test_unused_outputs_and_inputs():
+    """Gradients where only one of two outputs is used, where only some
+    inputs want one, and where the gradient is broadcast."""
+    gen = torch.Generator().manual_seed(21)
+    q = randn(gen, (2, 9, 4, 32), BF16, "cuda").requires_grad_(True)
+    k = randn(gen, (2, 9, 2, 32), BF16, "cuda").requires_grad_(True)
+    y, z = qk_norm_rope(q, k)
+    dq, dk = torch.autograd.grad(y.sum(), (q, k))
+    want, = torch.autograd.grad(qk_norm_rope(q, k.detach())[0].sum(), q)
+    assert torch.equal(dq, want) and not dk.any()
+    v = randn(gen, (2, 9, 2, 32), BF16, "cuda")
+    every = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    all_of = torch.autograd.grad(window_attention(*every).sum(), every)
+    for i in range(3):
+        some = [t.detach().requires_grad_(j == i)
+                for j, t in enumerate(every)]
+        one, = torch.autograd.grad(window_attention(*some).sum(), some[i])
+        assert torch.equal(one, all_of[i])
+
+
 # ---- offsets past 32 bits ----
 
 @gpu
