@@ -440,11 +440,6 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
             const int d = i * 16 + lane / 32 * 8;
             qop[i] = *(const s16x8 *)(row + (d < a.D ? d : 0));
         }
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const int d = i * 16 + lane / 32 * 8;
-            if (!live || d >= a.D) qop[i] = s16x8{};
-        }
     }
 
     const Tiles tl =
@@ -564,6 +559,10 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     if (i < end) {
         f32x16 xa[KT / 32], xb[KT / 32];
         kshare.send(kt0, kbase, a.ks, tl.at(i) * KT, s.n, wid, lane, a.D);
+        // the first tile is on its way before q is waited for
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            if (!live || d * 16 + lane / 32 * 8 >= a.D) qop[d] = s16x8{};
         ready(kt1, vt0);
         score(kt0, xa);
         settle(tl.at(i) * KT, xa);
@@ -702,7 +701,7 @@ __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 // and dk (at 2048 causal tokens 0.0025 of their norm, 0.0024 with it, where
 // the rounding of dq itself is 0.0017).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
+__global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
 {
     __shared__ Tile<DP> kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
@@ -727,7 +726,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
         (((long long)b * a.S + qi) * a.Hk * a.G + head) * a.D;
 
     s16x8 qop[DP / 16], gop[DP / 16];
-    float delta = 0.f;
+    typedef typename vec8<T>::type T8;
+    T8 o[DP / 16], rest[DP / 16];
     {
         const int rr = r < SG ? r : SG - 1, i = rr / a.G;
         const int hh = h * a.G + rr - i * a.G;
@@ -737,8 +737,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
                             (long long)hh * a.gh;
         const long long at =
             (((long long)b * a.S + i) * a.Hk * a.G + hh) * a.D;
-        typedef typename vec8<T>::type T8;
-        T8 o[DP / 16], rest[DP / 16];
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             int d = i * 16 + lane / 32 * 8;
@@ -748,19 +746,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
             rest[i] = *(const T8 *)((const T *)a.orest + at + d);
             qop[i] = *(const s16x8 *)(qrow + d);
         }
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const int d = i * 16 + lane / 32 * 8;
-            if (!live || d >= a.D) qop[i] = gop[i] = s16x8{};
-            const T8 z = __builtin_bit_cast(T8, gop[i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                delta += ((float)o[i][j] + (float)rest[i][j]) * (float)z[j];
-        }
     }
-    delta += other_half(delta);
-    const float lse = r < SG ? a.lse[row] : __builtin_inff();
-    if (r < SG && lane < 32) a.delta[row] = delta;
+    const float kept = a.lse[(long long)bh * SG + (r < SG ? r : SG - 1)];
 
     const Tiles tl =
         tiles_of(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
@@ -778,6 +765,21 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
         kshare.send(kt, kbase, a.ks, tile * KT, s.n, wid, lane, a.D);
         vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
     };
+    // the first tiles are on their way before the rows are waited for
+    if (end > 0) send(tl.at(0), kt0, vt0);
+    float delta = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        if (!live || i * 16 + lane / 32 * 8 >= a.D)
+            qop[i] = gop[i] = s16x8{};
+        const T8 z = __builtin_bit_cast(T8, gop[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            delta += ((float)o[i][j] + (float)rest[i][j]) * (float)z[j];
+    }
+    delta += other_half(delta);
+    const float lse = r < SG ? kept : __builtin_inff();
+    if (r < SG && lane < 32) a.delta[row] = delta;
     int i = 0;
     auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
                     Tile<DP> &vn) {
@@ -817,7 +819,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const Args a)
             }
         }
     };
-    if (i < end) send(tl.at(i), kt0, vt0);
     // two buffers by name, so that reads of one are known not to touch
     // what is on its way into the other
     while (i < end) {
@@ -874,7 +875,7 @@ struct RowData {
 // `splits_rows` rows whose f32 sums attn_join_kv adds in order, and so are
 // the others where there are few blocks.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attn_dkv(const Args a)
+__global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
 {
     __shared__ Tile<DP> qt0, qt1, gt0, gt1;
     __shared__ RowData rd0, rd1;
