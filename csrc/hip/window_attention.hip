@@ -633,8 +633,54 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         a.lse[row] = l == 0.f ? __builtin_inff() : m * a.c + log2f(l);
 }
 
-// Joins the parts of a row, one block a row: each wave a quarter of them
-// in order, against the quarter's own maximum, then the quarters in order.
+// Joins the parts of a row where they are few: four columns a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_few(const Args a)
+{
+    constexpr int PER = DP / 4;
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = e / PER;
+    const int c = (int)(e - row * PER) * 4;
+    if (row >= (long long)a.B * a.Hk * a.S * a.G) return;
+    const float *ml = a.part_ml + row * a.splits * 2;
+    float m = -__builtin_inff();
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[2 * i]);
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    float l = 0.f;
+    f32x4 x = {};
+    const float *po = a.part_o + row * a.splits * DP + c;
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) {
+        const float w = __builtin_amdgcn_exp2f(ml[2 * i] - base);
+        l += w * ml[2 * i + 1];
+        x += w * *(const f32x4 *)(po + (long long)i * DP);
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const long long bh = row / (a.S * a.G);
+    const int r = (int)(row - bh * (a.S * a.G)), qi = r / a.G;
+    const int g = r - qi * a.G;
+    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
+    const long long at =
+        (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D + c;
+    if (c < a.D) {
+        typedef __attribute__((ext_vector_type(4))) T T4;
+        T4 y, z;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = x[j] * inv;
+            y[j] = (T)f;
+            z[j] = (T)(f - (float)y[j]);
+        }
+        *(T4 *)((T *)a.out + at) = y;
+        if (a.rest) *(T4 *)((T *)a.rest + at) = z;
+    }
+    if (a.lse && c == 0)
+        a.lse[row] = l == 0.f ? __builtin_inff() : base + log2f(l);
+}
+
+// Joins the parts of a row where they are many, one block a row: each wave
+// a quarter of them in order, against the quarter's own maximum, then the quarters in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 {
@@ -851,15 +897,36 @@ __device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
     if (p1 > s.start + a.S - 1) p1 = s.start + a.S - 1;
 }
 
-// Parts of key block k0 that hold anything for the 32 keys from w0: where
-// those are past the first tokens, no more than reach to the end of the
-// last key's window.
-__device__ inline int parts_of(const Args &a, int k0, int w0, int parts)
+// Rows [r0, r1) that see keys k0..k0+127, and into how many parts of
+// `piece` rows they are cut.
+struct KeyRows {
+    int r0, r1, piece, parts;
+};
+__device__ inline KeyRows key_rows(const Args &a, const Seq &s, int k0)
 {
-    if (k0 >= a.sinks || w0 < a.sinks) return parts;
+    KeyRows k = {0, 0, k0 < a.sinks && a.sink_blocks ? a.sink_rows
+                                                     : a.splits_rows,
+                 1};
+    int p0, p1;
+    rows_of(a, s, k0, k0 + 127, p0, p1);
+    if (p0 <= p1) {
+        k.r0 = (p0 - s.start) * a.G;
+        k.r1 = (p1 - s.start + 1) * a.G;
+        k.parts = (int)(((long long)k.r1 - k.r0 + k.piece - 1) / k.piece);
+    }
+    return k;
+}
+
+// Parts of it that hold anything for the 32 keys from w0: where those are
+// past the first tokens, no more than reach to the end of the last key's
+// window.
+__device__ inline int parts_of(const Args &a, const KeyRows &k, int k0,
+                               int w0)
+{
+    if (k0 >= a.sinks || w0 < a.sinks) return k.parts;
     const long long rows = ((long long)k0 + 127 + a.window) * a.G;
-    const long long n = (rows + a.sink_rows - 1) / a.sink_rows;
-    return n < parts ? (int)n : parts;
+    const long long n = (rows + k.piece - 1) / k.piece;
+    return n < k.parts ? (int)n : k.parts;
 }
 
 // What dk and dv need of a tile's rows.
@@ -884,17 +951,15 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
     const int heads = a.B * a.Hk;
-    int u = blockIdx.x / heads, blk, part, parts;
-    const int bh = blockIdx.x - u * heads;
+    int u = blockIdx.x / heads, blk, part;
+    const int bh = blockIdx.x - u * heads, slot = u;
     if (u < a.sink_blocks * a.sink_splits) {
-        parts = a.sink_splits;
-        blk = u / parts;
-        part = u - blk * parts;
+        blk = u / a.sink_splits;
+        part = u - blk * a.sink_splits;
     } else {
         u -= a.sink_blocks * a.sink_splits;
-        parts = a.splits;
-        blk = u / parts;
-        part = u - blk * parts;
+        blk = u / a.splits;
+        part = u - blk * a.splits;
         blk += a.sink_blocks;
     }
     const int b = bh / a.Hk, h = bh - b * a.Hk;
@@ -902,6 +967,11 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     const Seq s = sequence(a, b);
     const int k0 = blk * 128, w0 = k0 + wid * 32;
     const int key = w0 + lane % 32;
+    const KeyRows kr = key_rows(a, s, k0);
+    if (part >= kr.parts) return;  // the whole block
+    const long long from = kr.r0 + (long long)part * kr.piece;
+    const int r0 = (int)from;
+    const int r1 = kr.r1 - from > kr.piece ? r0 + kr.piece : kr.r1;
 
     s16x8 kop[DP / 16], vop[DP / 16];
     {
@@ -923,20 +993,6 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
             if (key >= s.n || d >= a.D) kop[i] = vop[i] = s16x8{};
         }
     }
-    int p0, p1;
-    rows_of(a, s, k0, k0 + 127, p0, p1);
-    int r0 = 0, r1 = 0;  // rows [r0, r1)
-    if (p0 <= p1) {
-        r0 = (p0 - s.start) * a.G;
-        r1 = (p1 - s.start + 1) * a.G;
-    }
-    if (parts > 1) {
-        const int piece = blk < a.sink_blocks ? a.sink_rows : a.splits_rows;
-        const long long x = r0 + (long long)part * piece;
-        r0 = x < r1 ? (int)x : r1;
-        if (part < parts - 1 && r1 - r0 > piece) r1 = r0 + piece;
-    }
-
     // the rows that see this lane's key, as positions
     int plo = 0, phi = -1;
     if (key < s.n) rows_of(a, s, key, key, plo, phi);
@@ -1079,14 +1135,8 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
         step(qt1, gt1, rd1, qt0, gt0, rd0);
         t0 += KT;
     }
-    if (parts > 1) {
-        if (key >= a.T || part >= parts_of(a, k0, w0, parts)) return;
-        // parts of a key head: sink blocks', then the others'
-        const long long slot =
-            blk < a.sink_blocks
-                ? (long long)blk * a.sink_splits + part
-                : (long long)a.sink_blocks * a.sink_splits +
-                      (long long)(blk - a.sink_blocks) * a.splits + part;
+    if (kr.parts > 1) {
+        if (key >= a.T || part >= parts_of(a, kr, k0, w0)) return;
         const long long at =
             (((long long)bh * units + slot) * 128 + (key - k0)) * DP;
 #pragma unroll
@@ -1116,60 +1166,50 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     store_row<T, DP>((T *)a.dv + at, dv, D, lane);
 }
 
-// Adds the parts of dk and dv, one block a key: each wave a quarter of the
-// parts in order, then the quarters in order.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kv(const Args a, int DP)
+// Adds the parts of dk and dv in order: four columns of a key a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
 {
-    __shared__ float part[4][2][128];
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
-    const int blocks = a.splits > 1 ? a.blocks : a.sink_blocks;
+    constexpr int PER = DP / 4;           // threads of a key
+    constexpr int EACH = 128 * PER / 256;  // workgroups of a block of keys
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
-    const int bh = blockIdx.x / (blocks * 128);
-    const int key = blockIdx.x - bh * blocks * 128;
-    if (key >= a.T) return;
-    const int blk = key / 128;
-    const bool sink = blk < a.sink_blocks;
-    int parts = sink ? a.sink_splits : a.splits;
-    if (parts == 1) return;  // written where it was summed
-    if (sink) parts = parts_of(a, blk * 128, key & ~31, parts);
-    const long long slot =
-        sink ? (long long)blk * a.sink_splits
-             : (long long)a.sink_blocks * a.sink_splits +
-                   (long long)(blk - a.sink_blocks) * a.splits;
-    const long long from =
-        (((long long)bh * units + slot) * 128 + key % 128) * DP;
-    const int p0 = parts * wid / 4, p1 = parts * (wid + 1) / 4;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int c = lane + j * WAVE;
-        float x = 0.f, y = 0.f;
-        if (c < a.D) {
-#pragma unroll 8
-            for (int i = p0; i < p1; ++i) {
-                x += a.part_k[from + (long long)i * 128 * DP + c];
-                y += a.part_v[from + (long long)i * 128 * DP + c];
-            }
-        }
-        part[wid][0][c] = x;
-        part[wid][1][c] = y;
-    }
-    __syncthreads();
-    const int c = threadIdx.x % 128, which = threadIdx.x / 128;
-    if (c >= a.D) return;
-    const float z = part[0][which][c] + part[1][which][c] +
-                    part[2][which][c] + part[3][which][c];
+    const int id = blockIdx.x / EACH, bh = id / blocks;
+    const int blk = id - bh * blocks, k0 = blk * 128;
+    const int e = (blockIdx.x - id * EACH) * 256 + threadIdx.x;
+    const int key = k0 + e / PER, c = e % PER * 4;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
+    const KeyRows kr = key_rows(a, sequence(a, b), k0);
+    if (kr.parts <= 1) return;  // written where it was summed
+    const int parts = parts_of(a, kr, k0, key & ~31);
+    const long long slot =
+        blk < a.sink_blocks
+            ? (long long)blk * a.sink_splits
+            : (long long)a.sink_blocks * a.sink_splits +
+                  (long long)(blk - a.sink_blocks) * a.splits;
+    const long long from = ((long long)bh * units + slot) * 128 * DP + e * 4;
+    f32x4 x = {}, y = {};
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+        x += *(const f32x4 *)(a.part_k + from + (long long)i * 128 * DP);
+        y += *(const f32x4 *)(a.part_v + from + (long long)i * 128 * DP);
+    }
+    if (key >= a.T || c >= a.D) return;
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    T4 k, v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        k[j] = (T)(x[j] * a.scale);
+        v[j] = (T)y[j];
+    }
     const long long at = (((long long)b * a.T + key) * a.Hk + h) * a.D + c;
-    if (which)
-        ((T *)a.dv)[at] = (T)z;
-    else
-        ((T *)a.dk)[at] = (T)(z * a.scale);
+    *(T4 *)((T *)a.dk + at) = k;
+    *(T4 *)((T *)a.dv + at) = v;
 }
 
 // ---- how the work is cut ----
 constexpr int CUS = 256;
+constexpr int FEW = 8;  // parts of a row that one thread still adds up
 
 inline int dp_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 
@@ -1211,33 +1251,40 @@ FwdPlan plan_fwd(const Args &a)
     return p;
 }
 
-// dk and dv: parts of at most as many rows as a block without first tokens
-// sees, shorter ones where the blocks are fewer than the places for them.
+// dk and dv: where there are fewer blocks of keys than places for them, the
+// rows that see a block are cut so that all places have one even share
+// (s8192, 16/4 heads of 128, no mask: 256 blocks for 512 places, 1924 us
+// uncut, 1131 us in halves). Where causal blocks of all lengths leave most
+// places idle behind the longest, they are cut in thirds of a share (b2
+// s4096, 16/4 heads of 128: 555 us in shares, 450 us in thirds), though the
+// sums then take more of the memory's time (38 us there).
 // The blocks with first tokens, which every row sees, are cut into eighths
-// of that, so that they fill up what the others leave at the end: 8192
-// tokens, 32/8 heads of 128, window 1024, has 504 blocks and 57 such
+// of the others' rows, so that they fill up what those leave at the end:
+// 8192 tokens, 32/8 heads of 128, window 1024, has 504 blocks and 57 such
 // eighths a head for 512 places.
 void plan_dkv(Args &a)
 {
     const long long SG = (long long)a.S * a.G;
+    const bool window = a.window < a.T;
     a.blocks = (a.T + 127) / 128;
     const long long sink =
-        a.window >= a.T ? 0
-                        : ((a.sinks < a.T ? a.sinks : a.T) + 127ll) / 128;
+        window ? ((a.sinks < a.T ? a.sinks : a.T) + 127ll) / 128 : 0;
     a.sink_blocks = (int)sink;
     long long rows =
-        a.window >= a.T
-            ? SG
-            : (127ll + (a.causal ? 1ll : 2ll) * a.window) * a.G;
+        window ? (127ll + (a.causal ? 1ll : 2ll) * a.window) * a.G : SG;
     if (rows > SG) rows = SG;
     const long long bh = (long long)a.B * a.Hk;
-    const long long all = bh * a.blocks;
+    const long long places = (a.D > 64 ? 2ll : 3ll) * CUS;
     auto tiles = [](long long n) {  // at least 256 rows, whole tiles
         n = n < 256 ? 256 : n;
         return (n + KT - 1) / KT * KT;
     };
+    // where causal and without a window, blocks see half of the rows
+    const long long each = a.causal && !window ? rows / 2 : rows;
+    const long long share = bh * a.blocks * each / places;
+    const bool cut = each < rows ? rows > 2 * share : rows > share;
     const long long piece =
-        tiles(all < 2 * CUS ? rows * all / (2 * CUS) : rows);
+        tiles(!cut ? rows : each < rows ? share / 3 : share);
     a.splits_rows = (int)piece;
     a.splits = (int)((rows + piece - 1) / piece);
     a.sink_rows = a.splits_rows;
@@ -1283,7 +1330,11 @@ hipError_t launch_fwd(Args &a, const FwdPlan &p, hipStream_t s)
     }
     if (p.splits > 1) {  // rows of few blocks, so few
         const long long rows = (long long)a.B * a.Hk * a.S * a.G;
-        attn_join<T><<<(unsigned)rows, 256, 0, s>>>(a, DP);
+        if (p.splits > FEW)
+            attn_join<T><<<(unsigned)rows, 256, 0, s>>>(a, DP);
+        else
+            attn_join_few<T, DP>
+                <<<(unsigned)((rows * (DP / 4) + 255) / 256), 256, 0, s>>>(a);
     }
     return hipGetLastError();
 }
@@ -1296,13 +1347,14 @@ hipError_t launch_bwd(Args &a, hipStream_t s)
     d.blocks = (int)((SG + 127) / 128);
     const long long n = bh * d.blocks, m = bh * kv_units(a);
     const bool parts = kv_parts(a);
-    const long long j =
-        parts ? bh * (a.splits > 1 ? a.blocks : a.sink_blocks) * 128 : 0;
+    const int joined = a.splits > 1 ? a.blocks : a.sink_blocks;
+    const long long j = parts ? bh * joined * (DP / 8) : 0;
     if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32 || j * 256 >= 1ll << 32)
         return hipErrorInvalidValue;
     if (n) attn_dq<T, DP><<<(unsigned)n, 256, 0, s>>>(d);
     attn_dkv<T, DP><<<(unsigned)m, 256, 0, s>>>(a);
-    if (parts) attn_join_kv<T><<<(unsigned)j, 256, 0, s>>>(a, DP);
+    if (parts)
+        attn_join_kv<T, DP><<<(unsigned)j, 256, 0, s>>>(a, joined);
     return hipGetLastError();
 }
 
