@@ -38,7 +38,8 @@ using namespace kfv;
 
 namespace {
 
-constexpr int KT = 64;  // rows of a streamed tile
+constexpr int TILE = 64;  // rows of a streamed tile
+constexpr int KT = TILE;
 
 struct Args {
     const void *q, *k, *v, *dout, *o, *orest;
@@ -135,11 +136,11 @@ __device__ inline s16x8 pack8(const f32x16 &x, int at)
 // chunks of a row are permuted instead, c to c ^ f(row) within blocks of BS
 // chunks. f takes neighbouring rows' pairs of chunks (the transposing
 // read) and eight rows' single chunks (the plain one) to distinct banks.
-template <int DP>
+template <int DP, int ROWS = KT>
 struct Tile {
     static constexpr int CH = DP / 8;                      // chunks of a row
     static constexpr int BS = DP == 128 ? 16 : DP == 64 ? 8 : 4;
-    __align__(1024) short x[KT * DP];
+    __align__(1024) short x[ROWS * DP];
 
     static __device__ inline int f(int row)
     {
@@ -160,8 +161,8 @@ __device__ inline int rows_at(int lane)
 {
     return Tile<DP>::at(lane % 32, lane / 32);
 }
-template <int DP>
-__device__ inline s16x8 rows_op(const Tile<DP> &t, int at, int r0, int ks)
+template <int DP, int ROWS>
+__device__ inline s16x8 rows_op(const Tile<DP, ROWS> &t, int at, int r0, int ks)
 {
     constexpr int BS = Tile<DP>::BS;
     const int c = ks * 2;
@@ -181,8 +182,8 @@ __device__ inline int cols_at(int lane)
                         lane / 16 % 2 * 2 + i % 4 / 2) +
            i % 2 * 8;
 }
-template <int DP>
-__device__ inline s16x8 cols_op(const Tile<DP> &t, int at, int r0, int dt)
+template <int DP, int ROWS>
+__device__ inline s16x8 cols_op(const Tile<DP, ROWS> &t, int at, int r0, int dt)
 {
     constexpr int BS = Tile<DP>::BS;
     const int c = dt * 4;
@@ -211,10 +212,10 @@ __device__ inline void send16(const void *from, void *to)
 
 // A lane's share of a tile that NW waves fill: which row and column its
 // v-th 16 bytes hold.
-template <int DP, int NW>
+template <int DP, int NW, int ROWS = KT>
 struct Share {
     static constexpr int CH = Tile<DP>::CH, BS = Tile<DP>::BS;
-    static constexpr int N = KT * CH / WAVE / NW;
+    static constexpr int N = ROWS * CH / WAVE / NW;
     static __device__ inline int row(int v, int wid, int lane)
     {
         return ((v * NW + wid) * WAVE + lane) / CH;
@@ -231,23 +232,23 @@ struct Share {
 // piece. Rows past the last one and columns past D repeat others, which
 // hold nothing that could not stand there: their scores are masked, their
 // weights are zeros, and their columns meet zeros or are not written.
-template <int DP, int NW, int U, typename At>
-__device__ inline void send_tile(Tile<DP> &t, int wid, At at)
+template <int DP, int NW, int U, int ROWS, typename At>
+__device__ inline void send_tile(Tile<DP, ROWS> &t, int wid, At at)
 {
 #pragma unroll U
-    for (int v = 0; v < Share<DP, NW>::N; ++v)
+    for (int v = 0; v < Share<DP, NW, ROWS>::N; ++v)
         send16(at(v), (char *)t.x + (v * NW + wid) * WAVE * 16);
 }
 
 // Byte offsets of a lane's pieces of a tile from its first row. Where the
 // waves' loads take whole rows, the v-th piece lies `step` bytes (the same
 // for all lanes) after the one before.
-template <int DP, int NW>
+template <int DP, int NW, int ROWS = KT>
 struct Offsets {
-    typedef Share<DP, NW> S;
+    typedef Share<DP, NW, ROWS> S;
     static constexpr bool WHOLE = NW * WAVE % S::CH == 0 &&
                                   NW * WAVE / S::CH % Tile<DP>::BS == 0;
-    static constexpr int ROWS = NW * WAVE / S::CH;  // of one v, if WHOLE
+    static constexpr int EACH = NW * WAVE / S::CH;  // rows of one v, if WHOLE
     unsigned off[WHOLE ? 1 : S::N];
     // row_off(row): elements of a row from the tile's first
     template <typename F>
@@ -258,8 +259,8 @@ struct Offsets {
             off[v] = 2u * (row_off(S::row(v, wid, lane)) +
                            S::col(v, wid, lane, D));
     }
-    // `step`: elements from a row to the one ROWS further
-    __device__ void send(Tile<DP> &t, const short *from, long long step,
+    // `step`: elements from a row to the one EACH further
+    __device__ void send(Tile<DP, ROWS> &t, const short *from, long long step,
                          int wid) const
     {
         send_tile<DP, NW, 16>(t, wid, [&](int v) {
@@ -272,26 +273,27 @@ struct Offsets {
 // Keys and values: rows j0.. of a [T][D] matrix. Whole tiles take the
 // lane's offsets, which are the same for all of them, on a base that is
 // the same for all lanes; the last tile of a sequence stops at its end.
-template <int DP, int NW>
+template <int DP, int NW, int ROWS = KT>
 struct KeyShare {
-    Offsets<DP, NW> o;
+    typedef Share<DP, NW, ROWS> S;
+    Offsets<DP, NW, ROWS> o;
     __device__ KeyShare(long long stride, int wid, int lane, int D)
     {
         o.set(wid, lane, D,
               [&](int row) { return (unsigned)row * (unsigned)stride; });
     }
-    __device__ void send(Tile<DP> &t, const short *base, long long stride,
+    __device__ void send(Tile<DP, ROWS> &t, const short *base, long long stride,
                          int j0, int end, int wid, int lane, int D) const
     {
-        if (j0 + KT <= end) {
-            o.send(t, base + j0 * stride, Offsets<DP, NW>::ROWS * stride,
+        if (j0 + ROWS <= end) {
+            o.send(t, base + j0 * stride, Offsets<DP, NW, ROWS>::EACH * stride,
                    wid);
         } else {
             send_tile<DP, NW, 1>(t, wid, [&](int v) {
-                int j = j0 + Share<DP, NW>::row(v, wid, lane);
+                int j = j0 + S::row(v, wid, lane);
                 j = j < end ? j : end - 1;
                 return base + j * stride +
-                       Share<DP, NW>::col(v, wid, lane, D);
+                       S::col(v, wid, lane, D);
             });
         }
     }
@@ -356,6 +358,7 @@ struct Tiles {
     __device__ int at(int i) const { return i < head ? i : from + i - head; }
 };
 
+template <int ROWS>
 __device__ inline Tiles tiles_of(const Args &a, const Seq &s, int p0, int p1)
 {
     Tiles t = {0, 0, 0};
@@ -366,9 +369,9 @@ __device__ inline Tiles tiles_of(const Args &a, const Seq &s, int p0, int p1)
     const int lo = x.lo < 0 ? 0 : x.lo;
     int hi = y.hi + 1;
     if (y.first > hi) hi = y.first;
-    t.from = lo / KT;
-    t.to = (hi + KT - 1) / KT;
-    const int sinks = (y.first + KT - 1) / KT;
+    t.from = lo / ROWS;
+    t.to = (hi + ROWS - 1) / ROWS;
+    const int sinks = (y.first + ROWS - 1) / ROWS;
     t.head = sinks < t.from ? sinks : t.from;
     return t;
 }
@@ -401,7 +404,12 @@ __device__ inline int seen(const Args &a, const Seq &s, int p0, int p1,
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
 {
-    __shared__ Tile<DP> kt0, kt1, vt0, vt1;
+    // One wave takes half the keys at a time, so that a CU holds four such
+    // blocks at 128 columns: 16 sequences of 5 to 16 thousand keys, 32/8
+    // heads, 131 us (5.3 TB/s) against 142 us.
+    constexpr int KT = NW == 1 ? 32 : TILE;
+    typedef Tile<DP, KT> Tile;
+    __shared__ Tile kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int heads = a.B * a.Hk;
@@ -443,7 +451,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     }
 
     const Tiles tl =
-        tiles_of(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
+        tiles_of<KT>(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
     int i = 0, end = tl.count();
     if (SPLIT) {
         const int n = end;
@@ -459,7 +467,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     float m = -__builtin_inff(), l = 0.f;
 
     int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
-    const KeyShare<DP, NW> kshare(a.ks, wid, lane, a.D),
+    const KeyShare<DP, NW, KT> kshare(a.ks, wid, lane, a.D),
         vshare(a.vs, wid, lane, a.D);
     // Step u computes the scores of tile u and, in the same run of
     // instructions, the weights and products of tile u - 1, so that the
@@ -467,7 +475,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     // 8192 tokens, 891 TFLOP/s against 847 with one tile after another. It
     // needs keys u and values u - 1 in LDS, and sends keys u + 1 and values
     // u on their way.
-    auto score = [&](const Tile<DP> &kt, f32x16(&x)[KT / 32]) {
+    auto score = [&](const Tile &kt, f32x16(&x)[KT / 32]) {
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) {
             x[t] = f32x16{};
@@ -477,7 +485,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
                                x[t]);
         }
     };
-    auto weigh = [&](const Tile<DP> &vt, f32x16(&x)[KT / 32]) {
+    auto weigh = [&](const Tile &vt, f32x16(&x)[KT / 32]) {
         const float base = m == -__builtin_inff() ? 0.f : m * a.c;
         float sum[4] = {};
 #pragma unroll
@@ -532,7 +540,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     };
     // A tile that this wave sees nothing of, of those that its block sees,
     // is computed and masked as any other.
-    auto ready = [&](Tile<DP> &kn, Tile<DP> &vn) {
+    auto ready = [&](Tile &kn, Tile &vn) {
         landed();
         __syncthreads();
         if (i + 1 < end)
@@ -541,8 +549,8 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
         if (i < end)
             vshare.send(vn, vbase, a.vs, tl.at(i) * KT, s.n, wid, lane, a.D);
     };
-    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
-                    Tile<DP> &vn, f32x16(&xp)[KT / 32],
+    auto step = [&](const Tile &kt, const Tile &vt, Tile &kn,
+                    Tile &vn, f32x16(&xp)[KT / 32],
                     f32x16(&x)[KT / 32]) {
         ready(kn, vn);
         // the places that follow from these two are worked out again: kept,
@@ -796,7 +804,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     const float kept = a.lse[(long long)bh * SG + (r < SG ? r : SG - 1)];
 
     const Tiles tl =
-        tiles_of(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
+        tiles_of<KT>(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
     const int end = tl.count();
     const short *kbase = (const short *)a.k + b * a.kb + h * a.kh;
     const short *vbase = (const short *)a.v + b * a.vb + h * a.vh;
@@ -1006,7 +1014,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     // are the same queries and heads of every tile, at the same offsets
     // from its first query.
     typedef Offsets<DP, 4> Off;
-    const bool even = a.even && Off::ROWS % a.G == 0;
+    const bool even = a.even && Off::EACH % a.G == 0;
     Off qo, go;
     if (even) {
         qo.set(wid, lane, a.D, [&](int row) {
@@ -1025,7 +1033,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     // a row past the last one repeats it: its lse takes its weight to 0
     auto send = [&](int t0, Tile<DP> &qt, Tile<DP> &gt, RowData &rd) {
         if (even && t0 + KT <= r1) {
-            const int qi = t0 / a.G, step = Off::ROWS / a.G;
+            const int qi = t0 / a.G, step = Off::EACH / a.G;
             qo.send(qt, qbase + qi * a.qs, step * a.qs, wid);
             go.send(gt, gbase + qi * a.gs, step * a.gs, wid);
         } else {
