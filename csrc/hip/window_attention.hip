@@ -50,6 +50,7 @@ struct Args {
     int window, sinks, causal;
     const int *lengths, *starts;
     float scale, c;  // c = scale * log2(e)
+    int keys;        // of a block of dk and dv
     int blocks;      // row blocks (or key blocks) of a key head
     int splits;
     float *part_o, *part_ml;     // forward, split over keys
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     // One wave takes half the keys at a time, so that a CU holds four such
     // blocks at 128 columns: 16 sequences of 5 to 16 thousand keys, 32/8
     // heads, 131 us (5.3 TB/s) against 142 us.
-    constexpr int KT = NW == 1 ? 32 : TILE;
+    constexpr int KT = NW < 4 ? 32 : TILE;
     typedef Tile<DP, KT> Tile;
     __shared__ Tile kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
@@ -754,10 +755,13 @@ __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 // the rounding of 16 bits in it alone would add a tenth to the error of dq
 // and dk (at 2048 causal tokens 0.0025 of their norm, 0.0024 with it, where
 // the rounding of dq itself is 0.0017).
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
+template <typename T, int DP, int NW>
+__global__
+__launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
 {
-    __shared__ Tile<DP> kt0, kt1, vt0, vt1;
+    constexpr int KT = NW < 4 ? 32 : TILE;
+    typedef Tile<DP, KT> Tile;
+    __shared__ Tile kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int heads = a.B * a.Hk, unit = blockIdx.x / heads;
@@ -765,8 +769,8 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
-    const int r0 = blk * 128, w0 = r0 + wid * 32;
-    const int rlast = r0 + 128 < SG ? r0 + 127 : SG - 1;
+    const int r0 = blk * NW * 32, w0 = r0 + wid * 32;
+    const int rlast = r0 + NW * 32 < SG ? r0 + NW * 32 - 1 : SG - 1;
     const int wlast = w0 + 31 < SG ? w0 + 31 : SG - 1;
     const int r = w0 + lane % 32, qi = r / a.G, g = r - qi * a.G;
     const int p = s.start + qi;
@@ -813,9 +817,9 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
 
     const int rat = rows_at<DP>(lane), cat = cols_at<DP>(lane);
-    const KeyShare<DP, 4> kshare(a.ks, wid, lane, a.D),
+    const KeyShare<DP, NW, KT> kshare(a.ks, wid, lane, a.D),
         vshare(a.vs, wid, lane, a.D);
-    auto send = [&](int tile, Tile<DP> &kt, Tile<DP> &vt) {
+    auto send = [&](int tile, Tile &kt, Tile &vt) {
         kshare.send(kt, kbase, a.ks, tile * KT, s.n, wid, lane, a.D);
         vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
     };
@@ -835,8 +839,8 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     const float lse = r < SG ? kept : __builtin_inff();
     if (r < SG && lane < 32) a.delta[row] = delta;
     int i = 0;
-    auto step = [&](const Tile<DP> &kt, const Tile<DP> &vt, Tile<DP> &kn,
-                    Tile<DP> &vn) {
+    auto step = [&](const Tile &kt, const Tile &vt, Tile &kn,
+                    Tile &vn) {
         const int k0 = tl.at(i) * KT;
         landed();
         __syncthreads();
@@ -905,7 +909,7 @@ __device__ inline void rows_of(const Args &a, const Seq &s, int k0, int k1,
     if (p1 > s.start + a.S - 1) p1 = s.start + a.S - 1;
 }
 
-// Rows [r0, r1) that see keys k0..k0+127, and into how many parts of
+// Rows [r0, r1) that see the block of keys from k0, and into how many parts of
 // `piece` rows they are cut.
 struct KeyRows {
     int r0, r1, piece, parts;
@@ -916,7 +920,7 @@ __device__ inline KeyRows key_rows(const Args &a, const Seq &s, int k0)
                                                      : a.splits_rows,
                  1};
     int p0, p1;
-    rows_of(a, s, k0, k0 + 127, p0, p1);
+    rows_of(a, s, k0, k0 + a.keys - 1, p0, p1);
     if (p0 <= p1) {
         k.r0 = (p0 - s.start) * a.G;
         k.r1 = (p1 - s.start + 1) * a.G;
@@ -932,12 +936,13 @@ __device__ inline int parts_of(const Args &a, const KeyRows &k, int k0,
                                int w0)
 {
     if (k0 >= a.sinks || w0 < a.sinks) return k.parts;
-    const long long rows = ((long long)k0 + 127 + a.window) * a.G;
+    const long long rows = ((long long)k0 + a.keys + a.window) * a.G;
     const long long n = (rows + k.piece - 1) / k.piece;
     return n < k.parts ? (int)n : k.parts;
 }
 
 // What dk and dv need of a tile's rows.
+template <int KT>
 struct RowData {
     __align__(16) float lse[KT];
     __align__(16) float delta[KT];
@@ -949,10 +954,14 @@ struct RowData {
 // with first tokens are seen by all rows: they are split into parts of
 // `splits_rows` rows whose f32 sums attn_join_kv adds in order, and so are
 // the others where there are few blocks.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
+template <typename T, int DP, int NW>
+__global__
+__launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
 {
-    __shared__ Tile<DP> qt0, qt1, gt0, gt1;
+    constexpr int KT = NW < 4 ? 32 : TILE;
+    typedef Tile<DP, KT> Tile;
+    typedef RowData<KT> RowData;
+    __shared__ Tile qt0, qt1, gt0, gt1;
     __shared__ RowData rd0, rd1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -973,7 +982,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
-    const int k0 = blk * 128, w0 = k0 + wid * 32;
+    const int k0 = blk * NW * 32, w0 = k0 + wid * 32;
     const int key = w0 + lane % 32;
     const KeyRows kr = key_rows(a, s, k0);
     if (part >= kr.parts) return;  // the whole block
@@ -1013,8 +1022,9 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     // Where G divides the rows that the waves load at once, a lane's rows
     // are the same queries and heads of every tile, at the same offsets
     // from its first query.
-    typedef Offsets<DP, 4> Off;
-    const bool even = a.even && Off::EACH % a.G == 0;
+    typedef Offsets<DP, NW, KT> Off;
+    typedef Share<DP, NW, KT> Mine;
+    const bool even = a.even && (!Off::WHOLE || Off::EACH % a.G == 0);
     Off qo, go;
     if (even) {
         qo.set(wid, lane, a.D, [&](int row) {
@@ -1031,25 +1041,25 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     const short *gbase =
         (const short *)a.dout + b * a.gb + (long long)h * a.G * a.gh;
     // a row past the last one repeats it: its lse takes its weight to 0
-    auto send = [&](int t0, Tile<DP> &qt, Tile<DP> &gt, RowData &rd) {
+    auto send = [&](int t0, Tile &qt, Tile &gt, RowData &rd) {
         if (even && t0 + KT <= r1) {
             const int qi = t0 / a.G, step = Off::EACH / a.G;
             qo.send(qt, qbase + qi * a.qs, step * a.qs, wid);
             go.send(gt, gbase + qi * a.gs, step * a.gs, wid);
         } else {
             auto row = [&](int v) {
-                const int r = t0 + Share<DP, 4>::row(v, wid, lane);
+                const int r = t0 + Mine::row(v, wid, lane);
                 return r < r1 ? r : r1 - 1;
             };
-            send_tile<DP, 4, 1>(qt, wid, [&](int v) {
+            send_tile<DP, NW, 1>(qt, wid, [&](int v) {
                 const int r = row(v), qi = r / a.G, g = r - qi * a.G;
                 return qbase + qi * a.qs + g * a.qh +
-                       Share<DP, 4>::col(v, wid, lane, a.D);
+                       Mine::col(v, wid, lane, a.D);
             });
-            send_tile<DP, 4, 1>(gt, wid, [&](int v) {
+            send_tile<DP, NW, 1>(gt, wid, [&](int v) {
                 const int r = row(v), qi = r / a.G, g = r - qi * a.G;
                 return gbase + qi * a.gs + g * a.gh +
-                       Share<DP, 4>::col(v, wid, lane, a.D);
+                       Mine::col(v, wid, lane, a.D);
             });
         }
         if (wid == 0) {
@@ -1061,14 +1071,16 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
                 d = a.delta[(long long)bh * SG + r];
                 p = s.start + r / a.G;
             }
-            rd.lse[lane] = l;
-            rd.delta[lane] = d;
-            rd.pos[lane] = p;
+            if (lane < KT) {
+                rd.lse[lane] = l;
+                rd.delta[lane] = d;
+                rd.pos[lane] = p;
+            }
         }
     };
     int t0 = r0;
-    auto step = [&](const Tile<DP> &qt, const Tile<DP> &gt,
-                    const RowData &rd, Tile<DP> &qn, Tile<DP> &gn,
+    auto step = [&](const Tile &qt, const Tile &gt,
+                    const RowData &rd, Tile &qn, Tile &gn,
                     RowData &rn) {
         landed();
         __syncthreads();
@@ -1146,7 +1158,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     if (kr.parts > 1) {
         if (key >= a.T || part >= parts_of(a, kr, k0, w0)) return;
         const long long at =
-            (((long long)bh * units + slot) * 128 + (key - k0)) * DP;
+            (((long long)bh * units + slot) * NW * 32 + (key - k0)) * DP;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -1179,12 +1191,12 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
 {
     constexpr int PER = DP / 4;           // threads of a key
-    constexpr int EACH = 128 * PER / 256;  // workgroups of a block of keys
+    const int each = a.keys * PER / 256;   // workgroups of a block of keys
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
-    const int id = blockIdx.x / EACH, bh = id / blocks;
-    const int blk = id - bh * blocks, k0 = blk * 128;
-    const int e = (blockIdx.x - id * EACH) * 256 + threadIdx.x;
+    const int id = blockIdx.x / each, bh = id / blocks;
+    const int blk = id - bh * blocks, k0 = blk * a.keys;
+    const int e = (blockIdx.x - id * each) * 256 + threadIdx.x;
     const int key = k0 + e / PER, c = e % PER * 4;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const KeyRows kr = key_rows(a, sequence(a, b), k0);
@@ -1195,12 +1207,13 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
             ? (long long)blk * a.sink_splits
             : (long long)a.sink_blocks * a.sink_splits +
                   (long long)(blk - a.sink_blocks) * a.splits;
-    const long long from = ((long long)bh * units + slot) * 128 * DP + e * 4;
+    const long long part = (long long)a.keys * DP;
+    const long long from = ((long long)bh * units + slot) * part + e * 4;
     f32x4 x = {}, y = {};
 #pragma unroll 8
     for (int i = 0; i < parts; ++i) {
-        x += *(const f32x4 *)(a.part_k + from + (long long)i * 128 * DP);
-        y += *(const f32x4 *)(a.part_v + from + (long long)i * 128 * DP);
+        x += *(const f32x4 *)(a.part_k + from + i * part);
+        y += *(const f32x4 *)(a.part_v + from + i * part);
     }
     if (key >= a.T || c >= a.D) return;
     typedef __attribute__((ext_vector_type(4))) T T4;
@@ -1237,7 +1250,19 @@ struct FwdPlan {
     int waves, blocks, splits;
 };
 
-// Rows of a block: four waves of 32 share each key tile. Where that leaves
+// Whether blocks are of 64 rows or keys and tiles of 32, instead of 128 and
+// 64: what a block sees past each of its rows' windows is half as much,
+// which pays where that is a good part of it. 6 sequences of 1999 tokens,
+// 12 heads of 64, window 257, a training step: 136 us against 150; window
+// 512, 4 x 4096 tokens of 16 heads: 320 both; window 1024, forward: 96
+// against 94.
+bool narrow(const Args &a, long long n)
+{
+    return n > 128 && a.window < a.T &&
+           (a.causal ? 1ll : 2ll) * a.window <= 512;
+}
+
+// Rows of a block: four waves of 32, or two, share each key tile. Where that leaves
 // CUs without a block, blocks of one wave (when the rows fill no more),
 // and the keys are split until there are about four blocks a CU, with at
 // least four tiles each.
@@ -1245,7 +1270,7 @@ FwdPlan plan_fwd(const Args &a)
 {
     FwdPlan p;
     const long long SG = (long long)a.S * a.G;
-    p.waves = SG <= 32 ? 1 : 4;
+    p.waves = SG <= 32 ? 1 : narrow(a, SG) ? 2 : 4;
     p.blocks = (int)((SG + p.waves * 32 - 1) / (p.waves * 32));
     p.splits = 1;
     const long long all = (long long)p.blocks * a.B * a.Hk;
@@ -1274,15 +1299,20 @@ void plan_dkv(Args &a)
 {
     const long long SG = (long long)a.S * a.G;
     const bool window = a.window < a.T;
-    a.blocks = (a.T + 127) / 128;
+    // at 128 columns two waves' addresses would not fit the registers
+    a.keys = narrow(a, a.T) && a.D <= 64 ? 64 : 128;
+    a.blocks = (a.T + a.keys - 1) / a.keys;
     const long long sink =
-        window ? ((a.sinks < a.T ? a.sinks : a.T) + 127ll) / 128 : 0;
+        window
+            ? ((a.sinks < a.T ? a.sinks : a.T) + a.keys - 1ll) / a.keys
+            : 0;
     a.sink_blocks = (int)sink;
     long long rows =
-        window ? (127ll + (a.causal ? 1ll : 2ll) * a.window) * a.G : SG;
+        window ? (a.keys + (a.causal ? 1ll : 2ll) * a.window) * a.G : SG;
     if (rows > SG) rows = SG;
     const long long bh = (long long)a.B * a.Hk;
-    const long long places = (a.D > 64 ? 2ll : 3ll) * CUS;
+    const long long places =
+        (a.D > 64 ? 2ll : 3ll) * (a.keys == 64 ? 2 : 1) * CUS;
     auto tiles = [](long long n) {  // at least 256 rows, whole tiles
         n = n < 256 ? 256 : n;
         return (n + KT - 1) / KT * KT;
@@ -1330,6 +1360,11 @@ hipError_t launch_fwd(Args &a, const FwdPlan &p, hipStream_t s)
             attn_fwd<T, DP, 1, true><<<grid, 64, 0, s>>>(a);
         else
             attn_fwd<T, DP, 1, false><<<grid, 64, 0, s>>>(a);
+    } else if (p.waves == 2) {
+        if (p.splits > 1)
+            attn_fwd<T, DP, 2, true><<<grid, 128, 0, s>>>(a);
+        else
+            attn_fwd<T, DP, 2, false><<<grid, 128, 0, s>>>(a);
     } else {
         if (p.splits > 1)
             attn_fwd<T, DP, 4, true><<<grid, 256, 0, s>>>(a);
@@ -1352,15 +1387,23 @@ hipError_t launch_bwd(Args &a, hipStream_t s)
 {
     const long long SG = (long long)a.S * a.G, bh = (long long)a.B * a.Hk;
     Args d = a;
-    d.blocks = (int)((SG + 127) / 128);
+    const bool half = narrow(a, SG);
+    d.blocks = (int)(half ? (SG + 63) / 64 : (SG + 127) / 128);
     const long long n = bh * d.blocks, m = bh * kv_units(a);
     const bool parts = kv_parts(a);
     const int joined = a.splits > 1 ? a.blocks : a.sink_blocks;
-    const long long j = parts ? bh * joined * (DP / 8) : 0;
+    const long long j = parts ? bh * joined * (a.keys * (DP / 4) / 256) : 0;
     if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32 || j * 256 >= 1ll << 32)
         return hipErrorInvalidValue;
-    if (n) attn_dq<T, DP><<<(unsigned)n, 256, 0, s>>>(d);
-    attn_dkv<T, DP><<<(unsigned)m, 256, 0, s>>>(a);
+    if (half)
+        attn_dq<T, DP, 2><<<(unsigned)n, 128, 0, s>>>(d);
+    else
+        attn_dq<T, DP, 4><<<(unsigned)n, 256, 0, s>>>(d);
+    if (a.keys == 64)  // of at most 64 columns
+        attn_dkv<T, DP <= 64 ? DP : 64, 2>
+            <<<(unsigned)m, 128, 0, s>>>(a);
+    else
+        attn_dkv<T, DP, 4><<<(unsigned)m, 256, 0, s>>>(a);
     if (parts)
         attn_join_kv<T, DP><<<(unsigned)j, 256, 0, s>>>(a, joined);
     return hipGetLastError();
@@ -1414,7 +1457,7 @@ long long kf_attn_ws(const long long *dims, int backward)
     plan_dkv(a);
     long long n = (rows * 4 + 255) / 256 * 256;  // delta
     if (kv_parts(a))
-        n += 2ll * a.B * a.Hk * kv_units(a) * 128 * DP * 4;
+        n += 2ll * a.B * a.Hk * kv_units(a) * a.keys * DP * 4;
     return n;
 }
 
@@ -1492,13 +1535,13 @@ hipError_t kf_attn_bwd(const uintptr_t *ptrs, const long long *dims,
     a.scale = scale;
     a.c = scale * 1.44269504088896340736f;
     plan_dkv(a);
-    a.even = KT % a.G == 0 && near(a.qs * (KT / a.G) + a.qh * a.G) &&
+    a.even = 32 % a.G == 0 && near(a.qs * (KT / a.G) + a.qh * a.G) &&
              near(a.gs * (KT / a.G) + a.gh * a.G);
     const int DP = dp_of(a.D);
     const long long rows = (long long)a.B * a.Hk * a.S * a.G;
     a.delta = (float *)ptrs[12];
     a.part_k = a.delta + (rows * 4 + 255) / 256 * 64;
-    a.part_v = a.part_k + (long long)a.B * a.Hk * kv_units(a) * 128 * DP;
+    a.part_v = a.part_k + (long long)a.B * a.Hk * kv_units(a) * a.keys * DP;
     hipStream_t s = (hipStream_t)stream;
 #define CASE(N)                                                             \
     if (DP == N)                                                            \
