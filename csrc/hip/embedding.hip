@@ -149,7 +149,8 @@ __device__ inline unsigned block_scan(unsigned v, unsigned *wsum,
 
 // Few ids: block 0 sorts them all, keys and places in registers, one trip
 // through LDS for each digit; the other blocks clear the spans. 4096 ids of
-// 30522 tokens take 14 us, the passes below 35 us.
+// 30522 tokens take 14 us in one launch (the four launches below 21 us for
+// 14315 ids).
 __global__ __launch_bounds__(SMALL_BLOCK) void sort_small(
     const void *__restrict__ ids, int wide, int N, long long V,
     long long padding, int passes, int per, unsigned *__restrict__ keys,
