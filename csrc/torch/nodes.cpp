@@ -273,7 +273,10 @@ struct QKNormRope : Function<QKNormRope> {
         Tensor more[5] = {dense_rows(grads[0]), dense_rows(grads[1])};
         if (qw.defined()) more[2] = dense_like(qw);
         if (kw.defined()) more[3] = dense_like(kw);
-        if (q.size(2) + k.size(2) > 0) {
+        if (q.numel() == 0 && k.numel() == 0) {
+            for (int i = 2; i < 4; ++i)
+                if (more[i].defined()) more[i].zero_();
+        } else {
             if (qw.defined() || kw.defined())
                 more[4] = at::empty(
                     {(int64_t)K->qk_ws((int)q.size(3),

@@ -53,7 +53,7 @@ def _check(q, k, weights, rope, positions, start):
         if positions is not None:
             raise ValueError("positions without a rope table")
     else:
-        if rope.dim() != 2 or rope.shape[1] != D or \
+        if rope.dim() != 2 or rope.shape[1] != D or not rope.shape[0] or \
                 rope.dtype != torch.float32 or rope.device != q.device:
             raise ValueError("rope must be (positions, %d) float32 on %s" %
                              (D, q.device))

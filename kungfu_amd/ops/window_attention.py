@@ -118,7 +118,9 @@ def window_attention(q, k, v, window=None, sinks=0, causal=True,
 
     On the GPU: bf16 or f16 (f32 under autocast is cast as autocast says),
     a width that is a multiple of 8 up to 128. Probabilities are rounded to
-    that type for the product with v, all sums are f32.
+    that type for the product with v, and so are their gradients for the
+    products with q and k (in f16 those overflow past 65504); all sums are
+    f32.
     """
     if q.is_cuda and torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")

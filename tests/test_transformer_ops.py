@@ -280,6 +280,8 @@ def test_qk_refusals():
         (ValueError, (q, q, torch.ones(31)), {}),
         (TypeError, (q, q, torch.ones(32).double()), {}),
         (ValueError, (q, q, None, None, rope[:, :30]), {}),
+        (ValueError, (q, q, None, None, rope[:0]),
+         {"positions": torch.arange(4)}),
         (ValueError, (q, q, None, None, rope), {"start": 5}),
         (ValueError, (q, q, None, None, rope), {"start": -1}),
         (ValueError, (q, q), {"positions": torch.arange(4)}),
@@ -667,6 +669,74 @@ def test_unused_outputs_and_inputs():
                 for j, t in enumerate(every)]
         one, = torch.autograd.grad(window_attention(*some).sum(), some[i])
         assert torch.equal(one, all_of[i])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(0, 5), (3, 0)])
+def test_empty_batches(device, shape):
+    """No tokens: empty outputs, and zeros for what has a gradient."""
+    w = torch.randn(9, 16, device=device, requires_grad=True)
+    ids = torch.zeros(shape, dtype=torch.int64, device=device)
+    x = embedding(ids, w)
+    dw, = torch.autograd.grad(x.sum(), w)
+    assert x.shape == shape + (16,) and not dw.any()
+    q = torch.zeros(*shape, 2, 32, device=device, requires_grad=True)
+    a = torch.ones(32, device=device, requires_grad=True)
+    y, z = qk_norm_rope(q, q, a, a, rope_table(8, 32, device=device))
+    dq, da = torch.autograd.grad(y.sum() + z.sum(), (q, a))
+    assert y.shape == dq.shape == q.shape and not da.any()
+    h = torch.zeros(*shape, 2, 32, device=device, dtype=BF16)
+    h.requires_grad_(True)
+    dh, = torch.autograd.grad(window_attention(h, h, h).float().sum(), h)
+    assert dh.shape == h.shape
+
+
+@gpu
+def test_steps_free_what_they_kept():
+    a = block_inputs("cuda", BF16)
+    leaves = [t for t in a if t.requires_grad]
+
+    def step():
+        torch.autograd.grad(block(*a, 4).float().sum(), leaves)
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated()
+
+    step()
+    held = [step() for _ in range(4)]
+    assert len(set(held)) == 1
+
+
+@gpu
+def test_changed_inputs_are_noticed():
+    """A backward whose kept inputs were changed in place raises."""
+    q = torch.randn(1, 8, 2, 32, device="cuda").bfloat16()
+    x = q.clone().requires_grad_(True)
+    k = q.clone()
+    out = window_attention(x, k, q)
+    k.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.float().sum().backward()
+
+
+@gpu
+def test_lengths_and_positions_of_any_layout():
+    """int64 and int32, strided, far out of range."""
+    gen = torch.Generator().manual_seed(22)
+    q = randn(gen, (4, 40, 2, 64), BF16, "cuda")
+    want = window_attention(q, q, q, lengths=torch.tensor(
+        [40, 0, 7, 0], dtype=torch.int32, device="cuda"))
+    far = torch.tensor([[1 << 40, 9], [-(1 << 40), 9], [7, 9], [0, 9]],
+                       device="cuda")
+    assert torch.equal(want, window_attention(q, q, q, lengths=far[:, 0]))
+    starts = torch.tensor([0, 0, 0, 1 << 40], device="cuda")
+    got = window_attention(q, q, q, starts=starts)
+    assert torch.equal(got[:3], window_attention(q[:3], q[:3], q[:3]))
+    assert not got[3].any()
+    rope = rope_table(90, 64, device="cuda")
+    at = torch.randint(0, 90, (40, 4), generator=gen).cuda()
+    y = qk_norm_rope(q, q, rope=rope, positions=at.t())[0]
+    assert torch.equal(y, qk_norm_rope(q, q, rope=rope, positions=at.t()
+                                       .contiguous().int())[0])
 
 
 # ---- offsets past 32 bits ----
