@@ -42,15 +42,16 @@ __device__ inline unsigned load_key(const void *ids, int wide, long long n,
 // ---- forward ----
 // A block takes `rows` consecutive ids; its threads run over their vectors
 // of eight columns (VEC) or their columns one by one (rows that are not
-// 16-byte aligned), so that neighbours always touch neighbouring bytes, four
-// pieces at a time: the ids' loads go out together, and then the rows'.
+// 16-byte aligned), so that neighbours always touch neighbouring bytes,
+// several pieces at a time: the ids' loads go out together, and then the
+// rows'.
 template <typename W, typename O, bool VEC>
 __global__ __launch_bounds__(BLOCK) void embed_fwd(
     const void *__restrict__ ids, int wide, const W *__restrict__ weight,
     long long ldw, O *__restrict__ out, long long N, long long V, int H,
     int rows, float scale)
 {
-    constexpr int U = 4, E = VEC ? 8 : 1;
+    constexpr int U = VEC ? 4 : 8, E = VEC ? 8 : 1;
     const int per = H / E;
     for (long long n0 = (long long)blockIdx.x * rows; n0 < N;
          n0 += (long long)gridDim.x * rows) {
@@ -576,8 +577,9 @@ hipError_t fwd(const void *ids, int wide, const void *weight, long long ldw,
     const bool vec = H % 8 == 0 && ldw % 8 == 0 && aligned16(weight) &&
                      aligned16(out);
     const int per = vec ? H / 8 : H;
-    // about four vectors a thread
-    const int rows = per >= 4 * BLOCK ? 1 : 4 * BLOCK / per;
+    // one turn of a block's threads, or a row
+    const int turn = (vec ? 4 : 8) * BLOCK;
+    const int rows = per >= turn ? 1 : turn / per;
     long long blocks = (N + rows - 1) / rows;
     if (blocks > 1 << 20) blocks = 1 << 20;
     if (vec)

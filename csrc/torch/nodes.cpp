@@ -5,7 +5,7 @@
 // attribute of a tensor is a call. Here the nodes are C++ over the kernels
 // of `_hip`, which come in a capsule (csrc/hip/kernel_api.h). Arguments are
 // checked in Python, in kungfu_amd/ops; what these entries take is right in
-// shape, type and device.
+// shape, type and device, of any strides.
 //
 // A node runs on the device and stream that its forward ran on, as the
 // engine arranges, so the stream's handle is kept from there.
@@ -75,7 +75,9 @@ void row_strides(const Tensor &t, std::vector<long long> &to)
         to.push_back(t.size(i) == 1 ? 0 : (long long)t.stride(i));
 }
 
-// t, or a copy, with dense rows that start at 16 bytes.
+// t (batch, length, heads, width), or a copy of it, whose rows are dense and
+// start at 16 bytes, as the kernels that load 16 bytes at a time need, and
+// whose tokens are near enough for 32-bit offsets within a tile.
 Tensor rows16(const Tensor &t)
 {
     const int64_t each = 16 / t.element_size();
@@ -401,11 +403,13 @@ struct WindowAttention : Function<WindowAttention> {
     }
 };
 
-Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v,
+Tensor window_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
                         const Maybe &lengths, const Maybe &starts,
                         int64_t window, int64_t sinks, bool causal,
                         double scale, int64_t stream)
 {
+    // copies, where there are any, are part of the autograd graph
+    const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
     const AttnArgs a = {window, sinks, causal, stream, scale};
     if (wants_grad({q, k, v}))
         return WindowAttention::apply(q, k, v, lengths, starts, a);

@@ -239,27 +239,6 @@ def stream_of(t):
     return _stream_now(t.get_device())
 
 
-def row_strides(t):
-    """Strides of the leading dimensions; 0 where the size is 1 (such a
-    stride is arbitrary and never used)."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
-
-
-def rows16(t):
-    """t, or a copy of it, whose rows are dense and start at 16 bytes, as
-    the kernels that load 16 bytes at a time need, and whose tokens
-    (dimension 1) are near enough for 32-bit offsets within a tile."""
-    if t.numel() == 0:
-        return t
-    each = 16 // t.element_size()
-    strides = row_strides(t)
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % each == 0 for s in strides) and strides[1] < 1 << 24:
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def check_ints(name, t, shapes, device):
     """An int32 or int64 tensor of one of the shapes, on the device."""
     if t.dtype not in (torch.int32, torch.int64):

@@ -139,7 +139,6 @@ def window_attention(q, k, v, window=None, sinks=0, causal=True,
         every = torch.ones((), dtype=torch.bool, device=q.device)
         q, k, v = (t.masked_fill(every, 0) for t in (q, k, v))
         return q + k.sum() + v.sum()
-    q, k, v = hip.rows16(q), hip.rows16(k), hip.rows16(v)
     if lengths is not None:
         lengths = _int32(lengths)
     if starts is not None:
