@@ -53,10 +53,10 @@ struct Args {
     int keys;        // of a block of dk and dv
     int blocks;      // row blocks (or key blocks) of a key head
     int splits;
-    float *part_o, *part_ml;     // forward, split over keys
+    float *part_o, *part_ml;     // forward and dq, split over keys
     float *part_k, *part_v;      // dk, dv, split over rows
     int sink_blocks, sink_splits, splits_rows, sink_rows;
-    int even;  // G divides KT and a tile's offsets of rows fit 32 bits
+    int even;  // G divides a tile's rows, whose offsets fit 32 bits
 };
 
 template <typename T>
@@ -119,6 +119,22 @@ __device__ inline void store_row(T *row, const f32x16 (&x)[DP / 32], int D,
             if (c < D) *(s16x8 *)(row + c) = y[i];
         }
     }
+}
+
+// The same as f32.
+template <int DP>
+__device__ inline void store_sums(float *row, const f32x16 (&x)[DP / 32],
+                                  int lane)
+{
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f32x4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = x[d][e * 4 + j];
+            *(f32x4 *)(row + d * 32 + e * 8 + lane / 32 * 4) = y;
+        }
 }
 
 // Eight accumulators, from `at`, as a 16-bit operand.
@@ -602,16 +618,7 @@ __global__ __launch_bounds__(NW *WAVE, 2) void attn_fwd(const Args a)
     if (SPLIT) {
         if (r >= SG) return;
         // rows of a head in order, parts of a row together
-        float *po = a.part_o + (row * a.splits + split) * DP;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f32x4 y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = o[d][e * 4 + j];
-                *(f32x4 *)(po + d * 32 + e * 8 + lane / 32 * 4) = y;
-            }
+        store_sums<DP>(a.part_o + (row * a.splits + split) * DP, o, lane);
         if (lane < 32) {
             float *ml = a.part_ml + (row * a.splits + split) * 2;
             ml[0] = m * a.c;
@@ -755,7 +762,9 @@ __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 // the rounding of 16 bits in it alone would add a tenth to the error of dq
 // and dk (at 2048 causal tokens 0.0025 of their norm, 0.0024 with it, where
 // the rounding of dq itself is 0.0017).
-template <typename T, int DP, int NW>
+// SPLIT: the block takes one of `splits` parts of the row block's tiles and
+// writes its f32 sums, for attn_join_dq.
+template <typename T, int DP, int NW, bool SPLIT>
 __global__
 __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
 {
@@ -764,8 +773,13 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     __shared__ Tile kt0, kt1, vt0, vt1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int heads = a.B * a.Hk, unit = blockIdx.x / heads;
-    const int bh = blockIdx.x - unit * heads, blk = a.blocks - 1 - unit;
+    const int heads = a.B * a.Hk;
+    int unit = blockIdx.x, split = 0;
+    if (SPLIT) {
+        unit /= a.splits;
+        split = blockIdx.x - unit * a.splits;
+    }
+    const int blk = a.blocks - 1 - unit / heads, bh = unit % heads;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const int SG = a.S * a.G;
     const Seq s = sequence(a, b);
@@ -809,7 +823,12 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
 
     const Tiles tl =
         tiles_of<KT>(a, s, s.start + r0 / a.G, s.start + rlast / a.G);
-    const int end = tl.count();
+    int i = 0, end = tl.count();
+    if (SPLIT) {
+        const int n = end;
+        i = (int)((long long)n * split / a.splits);
+        end = (int)((long long)n * (split + 1) / a.splits);
+    }
     const short *kbase = (const short *)a.k + b * a.kb + h * a.kh;
     const short *vbase = (const short *)a.v + b * a.vb + h * a.vh;
     f32x16 acc[DP / 32];
@@ -824,7 +843,7 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
         vshare.send(vt, vbase, a.vs, tile * KT, s.n, wid, lane, a.D);
     };
     // the first tiles are on their way before the rows are waited for
-    if (end > 0) send(tl.at(0), kt0, vt0);
+    if (i < end) send(tl.at(i), kt0, vt0);
     float delta = 0.f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
@@ -837,8 +856,7 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
     }
     delta += other_half(delta);
     const float lse = r < SG ? kept : __builtin_inff();
-    if (r < SG && lane < 32) a.delta[row] = delta;
-    int i = 0;
+    if (r < SG && lane < 32 && split == 0) a.delta[row] = delta;
     auto step = [&](const Tile &kt, const Tile &vt, Tile &kn,
                     Tile &vn) {
         const int k0 = tl.at(i) * KT;
@@ -890,8 +908,40 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dq(const Args a)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             acc[d][e] = live ? acc[d][e] * a.scale : 0.f;
+    if (SPLIT) {
+        if (r < SG) store_sums<DP>(a.part_o + (row * a.splits + split) * DP,
+                                   acc, lane);
+        return;
+    }
     // lanes without a row take part in the exchanges, and write nothing
     store_row<T, DP>((T *)a.dq + orow, acc, r < SG ? a.D : 0, lane);
+}
+
+// Adds the parts of dq in order: four columns of a row a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_dq(const Args a)
+{
+    constexpr int PER = DP / 4;
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = e / PER;
+    const int c = (int)(e - row * PER) * 4;
+    if (row >= (long long)a.B * a.Hk * a.S * a.G || c >= a.D) return;
+    const float *part = a.part_o + row * a.splits * DP + c;
+    f32x4 x = {};
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i)
+        x += *(const f32x4 *)(part + (long long)i * DP);
+    const long long bh = row / (a.S * a.G);
+    const int r = (int)(row - bh * (a.S * a.G)), qi = r / a.G;
+    const int g = r - qi * a.G;
+    const int b = (int)(bh / a.Hk), h = (int)(bh - (long long)b * a.Hk);
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    T4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (T)x[j];
+    *(T4 *)((T *)a.dq +
+            (((long long)b * a.S + qi) * a.Hk * a.G + h * a.G + g) * a.D +
+            c) = y;
 }
 
 // Rows that see any of keys k0..k1, as positions [p0, p1].
@@ -1159,20 +1209,8 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
         if (key >= a.T || part >= parts_of(a, kr, k0, w0)) return;
         const long long at =
             (((long long)bh * units + slot) * NW * 32 + (key - k0)) * DP;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c0 = d * 32 + e * 8 + lane / 32 * 4;
-                f32x4 y, z;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[j] = dk[d][e * 4 + j];
-                    z[j] = dv[d][e * 4 + j];
-                }
-                *(f32x4 *)(a.part_k + at + c0) = y;
-                *(f32x4 *)(a.part_v + at + c0) = z;
-            }
+        store_sums<DP>(a.part_k + at, dk, lane);
+        store_sums<DP>(a.part_v + at, dv, lane);
         return;
     }
     const long long at =
@@ -1246,7 +1284,7 @@ long long most_tiles(const Args &a, int rows)
     return (keys + KT - 1) / KT;
 }
 
-struct FwdPlan {
+struct RowPlan {
     int waves, blocks, splits;
 };
 
@@ -1262,23 +1300,28 @@ bool narrow(const Args &a, long long n)
            (a.causal ? 1ll : 2ll) * a.window <= 512;
 }
 
-// Rows of a block: four waves of 32, or two, share each key tile. Where that leaves
-// CUs without a block, blocks of one wave (when the rows fill no more),
-// and the keys are split until there are about four blocks a CU, with at
-// least four tiles each.
-FwdPlan plan_fwd(const Args &a)
+// Rows of a block: four waves of 32, or two, share each key tile; one where
+// the rows fill no more. Where most places for blocks are left idle, the
+// keys are split until there is a block for each, with at least eight tiles
+// (2048 causal tokens, 16 heads of 64, 256 blocks for 768 places: dq 58 us
+// whole, 36 + 7 us split and joined; with a window of 512 over 4096 tokens
+// of 8/2 heads 26 us whole, 26 + 5 us split) or, of one wave, four.
+RowPlan plan_rows(const Args &a, bool few)
 {
-    FwdPlan p;
+    RowPlan p;
     const long long SG = (long long)a.S * a.G;
-    p.waves = SG <= 32 ? 1 : narrow(a, SG) ? 2 : 4;
+    p.waves = few && SG <= 32 ? 1 : narrow(a, SG) ? 2 : 4;
     p.blocks = (int)((SG + p.waves * 32 - 1) / (p.waves * 32));
     p.splits = 1;
     const long long all = (long long)p.blocks * a.B * a.Hk;
     const long long tiles = most_tiles(a, p.waves * 32);
-    const int want = p.waves == 1 ? 4 * CUS : CUS;
-    if (all < want) {
-        long long n = (want + all - 1) / all;
-        if (n > tiles / 4) n = tiles / 4;
+    const int places =
+        (p.waves == 1 ? 4 : (a.D > 64 ? 2 : 3) * (p.waves == 2 ? 2 : 1)) *
+        CUS;
+    if (all < (p.waves == 1 ? places : places / 2)) {
+        long long n = (places + all - 1) / all;
+        const long long least = p.waves == 1 ? 4 : 8;
+        if (n > tiles / least) n = tiles / least;
         if (n > 1) p.splits = (int)n;
     }
     return p;
@@ -1350,7 +1393,7 @@ bool kv_parts(const Args &a)
 }
 
 template <typename T, int DP>
-hipError_t launch_fwd(Args &a, const FwdPlan &p, hipStream_t s)
+hipError_t launch_fwd(Args &a, const RowPlan &p, hipStream_t s)
 {
     const long long n = (long long)a.B * a.Hk * p.blocks * p.splits;
     if (n * 64 * p.waves >= 1ll << 32) return hipErrorInvalidValue;
@@ -1387,18 +1430,27 @@ hipError_t launch_bwd(Args &a, hipStream_t s)
 {
     const long long SG = (long long)a.S * a.G, bh = (long long)a.B * a.Hk;
     Args d = a;
-    const bool half = narrow(a, SG);
-    d.blocks = (int)(half ? (SG + 63) / 64 : (SG + 127) / 128);
-    const long long n = bh * d.blocks, m = bh * kv_units(a);
+    const RowPlan p = plan_rows(a, false);
+    d.blocks = p.blocks;
+    d.splits = p.splits;
+    const long long n = bh * d.blocks * d.splits, m = bh * kv_units(a);
     const bool parts = kv_parts(a);
     const int joined = a.splits > 1 ? a.blocks : a.sink_blocks;
     const long long j = parts ? bh * joined * (a.keys * (DP / 4) / 256) : 0;
     if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32 || j * 256 >= 1ll << 32)
         return hipErrorInvalidValue;
-    if (half)
-        attn_dq<T, DP, 2><<<(unsigned)n, 128, 0, s>>>(d);
-    else
-        attn_dq<T, DP, 4><<<(unsigned)n, 256, 0, s>>>(d);
+    if (p.splits > 1) {
+        if (p.waves == 2)
+            attn_dq<T, DP, 2, true><<<(unsigned)n, 128, 0, s>>>(d);
+        else
+            attn_dq<T, DP, 4, true><<<(unsigned)n, 256, 0, s>>>(d);
+        attn_join_dq<T, DP>
+            <<<(unsigned)((bh * SG * (DP / 4) + 255) / 256), 256, 0, s>>>(d);
+    } else if (p.waves == 2) {
+        attn_dq<T, DP, 2, false><<<(unsigned)n, 128, 0, s>>>(d);
+    } else {
+        attn_dq<T, DP, 4, false><<<(unsigned)n, 256, 0, s>>>(d);
+    }
     if (a.keys == 64)  // of at most 64 columns
         attn_dkv<T, DP <= 64 ? DP : 64, 2>
             <<<(unsigned)m, 128, 0, s>>>(a);
@@ -1451,11 +1503,13 @@ long long kf_attn_ws(const long long *dims, int backward)
     const long long rows = (long long)a.B * a.Hk * a.S * a.G;
     const int DP = dp_of(a.D);
     if (!backward) {
-        const FwdPlan p = plan_fwd(a);
+        const RowPlan p = plan_rows(a, true);
         return p.splits > 1 ? rows * p.splits * (DP + 2) * 4 : 0;
     }
     plan_dkv(a);
     long long n = (rows * 4 + 255) / 256 * 256;  // delta
+    const RowPlan p = plan_rows(a, false);
+    if (p.splits > 1) n += rows * p.splits * DP * 4;
     if (kv_parts(a))
         n += 2ll * a.B * a.Hk * kv_units(a) * a.keys * DP * 4;
     return n;
@@ -1484,7 +1538,7 @@ hipError_t kf_attn_fwd(const uintptr_t *ptrs, const long long *dims,
     if (!near(a.ks * KT) || !near(a.vs * KT)) return hipErrorInvalidValue;
     a.scale = scale;
     a.c = scale * 1.44269504088896340736f;
-    const FwdPlan p = plan_fwd(a);
+    const RowPlan p = plan_rows(a, true);
     a.blocks = p.blocks;
     a.splits = p.splits;
     const int DP = dp_of(a.D);
@@ -1540,7 +1594,9 @@ hipError_t kf_attn_bwd(const uintptr_t *ptrs, const long long *dims,
     const int DP = dp_of(a.D);
     const long long rows = (long long)a.B * a.Hk * a.S * a.G;
     a.delta = (float *)ptrs[12];
-    a.part_k = a.delta + (rows * 4 + 255) / 256 * 64;
+    const RowPlan p = plan_rows(a, false);
+    a.part_o = a.delta + (rows * 4 + 255) / 256 * 64;
+    a.part_k = a.part_o + (p.splits > 1 ? rows * p.splits * DP : 0);
     a.part_v = a.part_k + (long long)a.B * a.Hk * kv_units(a) * a.keys * DP;
     hipStream_t s = (hipStream_t)stream;
 #define CASE(N)                                                             \
