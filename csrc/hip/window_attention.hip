@@ -1224,17 +1224,20 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     store_row<T, DP>((T *)a.dv + at, dv, D, lane);
 }
 
-// Adds the parts of dk and dv in order: four columns of a key a thread.
+// Adds the parts of dk and dv: four columns of a key a thread, each wave of
+// a block a quarter of the parts in order, then the quarters in order.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
 {
     constexpr int PER = DP / 4;           // threads of a key
-    const int each = a.keys * PER / 256;   // workgroups of a block of keys
+    __shared__ f32x4 sums[4][2][WAVE];
+    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
+    const int each = a.keys * PER / WAVE;  // workgroups of a block of keys
     const int units =
         a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
     const int id = blockIdx.x / each, bh = id / blocks;
     const int blk = id - bh * blocks, k0 = blk * a.keys;
-    const int e = (blockIdx.x - id * each) * 256 + threadIdx.x;
+    const int e = (blockIdx.x - id * each) * WAVE + lane;
     const int key = k0 + e / PER, c = e % PER * 4;
     const int b = bh / a.Hk, h = bh - b * a.Hk;
     const KeyRows kr = key_rows(a, sequence(a, b), k0);
@@ -1248,22 +1251,27 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
     const long long part = (long long)a.keys * DP;
     const long long from = ((long long)bh * units + slot) * part + e * 4;
     f32x4 x = {}, y = {};
+    const int p1 = parts * (wid + 1) / 4;
 #pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
+    for (int i = parts * wid / 4; i < p1; ++i) {
         x += *(const f32x4 *)(a.part_k + from + i * part);
         y += *(const f32x4 *)(a.part_v + from + i * part);
     }
-    if (key >= a.T || c >= a.D) return;
-    typedef __attribute__((ext_vector_type(4))) T T4;
-    T4 k, v;
+    sums[wid][0][lane] = x;
+    sums[wid][1][lane] = y;
+    __syncthreads();
+    if (wid > 1 || key >= a.T || c >= a.D) return;
+    // wave 0 writes dk, wave 1 dv
+    x = sums[0][wid][lane];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        k[j] = (T)(x[j] * a.scale);
-        v[j] = (T)y[j];
-    }
+    for (int i = 1; i < 4; ++i) x += sums[i][wid][lane];
+    const float by = wid ? 1.f : a.scale;
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    T4 z;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = (T)(x[j] * by);
     const long long at = (((long long)b * a.T + key) * a.Hk + h) * a.D + c;
-    *(T4 *)((T *)a.dk + at) = k;
-    *(T4 *)((T *)a.dv + at) = v;
+    *(T4 *)((T *)(wid ? a.dv : a.dk) + at) = z;
 }
 
 // ---- how the work is cut ----
@@ -1292,12 +1300,12 @@ struct RowPlan {
 // 64: what a block sees past each of its rows' windows is half as much,
 // which pays where that is a good part of it. 6 sequences of 1999 tokens,
 // 12 heads of 64, window 257, a training step: 136 us against 150; window
-// 512, 4 x 4096 tokens of 16 heads: 320 both; window 1024, forward: 96
-// against 94.
+// 512, 4 x 4096 tokens of 16 heads: 320 both, one sequence of 8/2 heads,
+// forward: 22 against 18; window 1024, forward: 96 against 94.
 bool narrow(const Args &a, long long n)
 {
     return n > 128 && a.window < a.T &&
-           (a.causal ? 1ll : 2ll) * a.window <= 512;
+           (a.causal ? 1ll : 2ll) * a.window <= 384;
 }
 
 // Rows of a block: four waves of 32, or two, share each key tile; one where
@@ -1436,7 +1444,7 @@ hipError_t launch_bwd(Args &a, hipStream_t s)
     const long long n = bh * d.blocks * d.splits, m = bh * kv_units(a);
     const bool parts = kv_parts(a);
     const int joined = a.splits > 1 ? a.blocks : a.sink_blocks;
-    const long long j = parts ? bh * joined * (a.keys * (DP / 4) / 256) : 0;
+    const long long j = parts ? bh * joined * (a.keys * (DP / 4) / WAVE) : 0;
     if (n * 256 >= 1ll << 32 || m * 256 >= 1ll << 32 || j * 256 >= 1ll << 32)
         return hipErrorInvalidValue;
     if (p.splits > 1) {
