@@ -22,6 +22,12 @@
 // read from the same LDS tile by the transposing 64-bit read with the rows
 // in that order. No probability passes through LDS or between lanes.
 //
+// Long rows are bound by the matrix pipe, which the softmax's vector work
+// beside it keeps from its full rate: 2 x 8192 tokens, 16 heads, no mask,
+// forward 1096 us at 128 columns (1003 TFLOP/s) and 615 us at 64 (894), dq
+// 1579 us (1044) and 911 us (905), dk and dv 2239 us (982) and 1235 us
+// (890). Few rows over many keys are bound by the reads of k and v.
+//
 // The backward computes the scores twice, once for dq and once for dk and
 // dv, instead of adding dq with atomics: every output is written once by
 // one block in a fixed order, so results repeat bit by bit.
@@ -1300,7 +1306,7 @@ struct RowPlan {
 // 64: what a block sees past each of its rows' windows is half as much,
 // which pays where that is a good part of it. 6 sequences of 1999 tokens,
 // 12 heads of 64, window 257, a training step: 136 us against 150; window
-// 512, 4 x 4096 tokens of 16 heads: 320 both, one sequence of 8/2 heads,
+// 512, 4 x 4096 tokens of 16 heads: 320 both, 4096 tokens of 8/2 heads,
 // forward: 22 against 18; window 1024, forward: 96 against 94.
 bool narrow(const Args &a, long long n)
 {
