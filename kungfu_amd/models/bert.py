@@ -136,7 +136,14 @@ class Bert(nn.Module):
         if self._rope is None or self._rope.device != device:
             from kungfu_amd.ops.qk_norm_rope import rope_table
 
-            self._rope = rope_table(*self.rotary, device=device)
+            # a tensor of inference mode could not be trained with
+            with torch.inference_mode(False):
+                if device.type == "cuda" and \
+                        torch.cuda.is_current_stream_capturing():
+                    # there after a replay only: not for other calls
+                    return rope_table(*self.rotary, device=device)
+                # the copy waits, so that any stream can use it
+                self._rope = rope_table(*self.rotary).to(device)
         return self._rope
 
     def forward(self, ids, lengths=None):

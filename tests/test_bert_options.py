@@ -183,3 +183,37 @@ def test_step_in_a_graph():
             rel = float((f.float() - want[i].float()).norm() /
                         want[i].float().norm())
             assert rel < 0.02, rel
+
+
+def test_trains_after_inference_mode():
+    """The first call may be one of inference mode: what the model keeps of
+    it, the angles, serves training too."""
+    m = make(12, **EVERY)
+    x = ids_of(2, 9)
+    with torch.inference_mode():
+        seen = m(x)
+    out = m(x)
+    out.square().mean().backward()
+    assert torch.equal(out, seen)
+    assert all(p.grad is not None for p in m.parameters())
+
+
+@gpu
+def test_angles_of_a_captured_first_call_are_not_kept():
+    """What a graph computes is there after a replay only: a call outside
+    the graph makes its own."""
+    m = make(14, **EVERY).cuda()
+    device = m.tok.weight.device
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = m._angles(device)
+    eager = m._angles(device).clone()
+    assert m._angles(device) is m._angles(device)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        # 64-bit cosines and sines of two libraries, rounded once to f32
+        assert torch.allclose(held, eager, rtol=0, atol=2.0 ** -24)
+        assert float(eager[0, 0]) == 1.0
