@@ -123,6 +123,10 @@ class Bert(nn.Module):
         low = self.fused_ln and ids.is_cuda
         x = self._lookup(self.tok, ids, low)
         if self.pos is not None:
+            if self.fused_embed and ids.shape[1] > self.pos.num_embeddings:
+                # the lookup on the GPU would answer NaN
+                raise IndexError("%d tokens for %d positions" %
+                                 (ids.shape[1], self.pos.num_embeddings))
             pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
             x = x + self._lookup(self.pos, pos, low)
         if low:

@@ -198,6 +198,15 @@ def test_trains_after_inference_mode():
     assert all(p.grad is not None for p in m.parameters())
 
 
+def test_too_long_a_batch_is_refused():
+    """Also where the lookup itself would not raise, on the GPU."""
+    for options in (dict(fused_embed=True), EVERY):
+        m = make(13, **options)
+        m(ids_of(1, 64))
+        with pytest.raises((ValueError, IndexError), match="64"):
+            m(ids_of(1, 65))
+
+
 @gpu
 def test_angles_of_a_captured_first_call_are_not_kept():
     """What a graph computes is there after a replay only: a call outside
