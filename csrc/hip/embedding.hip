@@ -640,7 +640,7 @@ bool fits(long long N, long long V, int H)
 {
     return N >= 0 && N < 1ll << 30 && V > 0 && V < 1ll << 30 && H > 0 &&
            H <= 1 << 20 &&
-           (N / CHUNK + 1) * ((H + COLS - 1) / COLS) < 1ll << 30;
+           (N / CHUNK + 1) * ((H + COLS - 1) / COLS) <= 1ll << 25;
 }
 
 }  // namespace

@@ -702,7 +702,8 @@ __global__ __launch_bounds__(256) void attn_join_few(const Args a)
 }
 
 // Joins the parts of a row where they are many, one block a row: each wave
-// a quarter of them in order, against the quarter's own maximum, then the quarters in order.
+// a quarter of them in order, against the quarter's own maximum, then the
+// quarters in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join(const Args a, int DP)
 {
