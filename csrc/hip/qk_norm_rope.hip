@@ -202,7 +202,7 @@ struct Walk {
         }
     }
     // Row of the table; -1 for a position outside it, which is not
-    // followed: its rows are NaN.
+    // followed: its rows are NaN and have no gradient.
     __device__ long long position(const Args &a) const
     {
         long long pos = a.start + s;
@@ -222,6 +222,7 @@ struct Angles {
     template <typename W>
     __device__ void load(const Args &a, const W &w, int li)
     {
+        ok = true;
         if (!a.rope) return;
         const long long pos = w.position(a);
         ok = pos >= 0;
@@ -322,12 +323,14 @@ __global__ __launch_bounds__(BLOCK) void qk_bwd(const Args a)
             const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
             const float m = group_sum(t, L) / (float)a.D * r * r * r;
             if (on[u]) {
+                // a row at a position outside the table has no gradient,
+                // whatever it holds: zeros, and no part in the weights'
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    al[j] += gl[j] * lo[j] * r;
-                    ah[j] += gh[j] * hi[j] * r;
-                    gl[j] = gl[j] * wl[j] * r - lo[j] * m;
-                    gh[j] = gh[j] * wh[j] * r - hi[j] * m;
+                    al[j] += ang[u].ok ? gl[j] * lo[j] * r : 0.f;
+                    ah[j] += ang[u].ok ? gh[j] * hi[j] * r : 0.f;
+                    gl[j] = ang[u].ok ? gl[j] * wl[j] * r - lo[j] * m : 0.f;
+                    gh[j] = ang[u].ok ? gh[j] * wh[j] * r - hi[j] * m : 0.f;
                 }
                 store_pairs<T, VEC>(out[u], gl, gh, half, li, L);
             }

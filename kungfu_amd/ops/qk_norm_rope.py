@@ -113,7 +113,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, rope=None,
     The width is even and at most 512. Without `positions` the range is
     checked here. A position in `positions` outside the table raises on the
     CPU; on the GPU, where reading it back would hold up the stream, the
-    rows at it are NaN.
+    rows at it are NaN, get zeros as gradients and add to none.
     """
     start, eps = int(start), float(eps)
     _check(q, k, (q_weight, k_weight), rope, positions, start)
