@@ -90,14 +90,18 @@ Tensor rows16(const Tensor &t)
     return ptr(c) % 16 == 0 ? c : c.clone();
 }
 
-// Gradients that are constants of a second differentiation: one asked for
-// raises, instead of being zero without a word.
-variable_list once(variable_list grads)
+// Gradients that cannot be differentiated again. Where they are made for
+// that, they hang on a node that raises, and the node on all of `from`: what
+// they were computed from. Any way through the operator to a leaf then
+// raises, instead of adding nothing without a word; ways past it stay open.
+variable_list once(variable_list grads, const variable_list &from)
 {
     if (!at::GradMode::is_enabled()) return grads;
     variable_list in;
     for (const auto &g : grads)
-        if (g.defined()) in.push_back(g.detach().requires_grad_(true));
+        if (g.defined()) in.push_back(g);
+    for (const auto &t : from)
+        if (t.defined() && t.requires_grad()) in.push_back(t);
     auto error = std::make_shared<torch::autograd::DelayedError>(
         "this operator has no second derivative", (int64_t)in.size());
     const variable_list out = (*error)(std::move(in));
@@ -178,7 +182,8 @@ struct Embedding : Function<Embedding> {
                            (float)d["scale"].toDouble(), ws.data_ptr(),
                            (void *)d["stream"].toInt()),
               "embedding backward");
-        return once({Tensor(), dw, Tensor()});
+        // linear in dout, and no function of the weight
+        return once({Tensor(), dw, Tensor()}, grads);
     }
 };
 
@@ -286,7 +291,8 @@ struct QKNormRope : Function<QKNormRope> {
                     q.options().dtype(at::kFloat));
             qk_launch(q, k, qw, kw, s[4], s[5], dq, dk, a, more);
         }
-        return once({dq, dk, more[2], more[3], Tensor(), Tensor(), Tensor()});
+        return once({dq, dk, more[2], more[3], Tensor(), Tensor(), Tensor()},
+                    {q, k, qw, kw, grads[0], grads[1]});
     }
 };
 
@@ -399,7 +405,8 @@ struct WindowAttention : Function<WindowAttention> {
         check(K->attn_bwd(ptrs, dims.data(), strides.data(), (float)a.scale,
                           type_code(q.scalar_type()), (void *)a.stream),
               "window_attention backward");
-        return once({dq, dk, dv, Tensor(), Tensor(), Tensor()});
+        return once({dq, dk, dv, Tensor(), Tensor(), Tensor()},
+                    {q, k, v, grads[0]});
     }
 };
 

@@ -1,12 +1,15 @@
-"""Calls of the transformer operators that differ from the plain ones: rows
-at positions outside the table, derivatives and traces that the operators
-do not have, checkpoints, workspaces of unusual plans."""
+"""Calls of the transformer operators at the edge of what they are for:
+derivatives that they do not have, rows at positions outside the table."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from kungfu_amd.ops import hip
+from kungfu_amd.ops.fused_embedding import embedding
 from kungfu_amd.ops.qk_norm_rope import qk_norm_rope, rope_table
+from kungfu_amd.ops.window_attention import window_attention
 
 gpu = pytest.mark.gpu
 BF16, F16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -14,6 +17,112 @@ BF16, F16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 def randn(gen, shape, dtype, device):
     return torch.randn(shape, generator=gen).to(dtype).to(device)
+
+
+# ---- the operators as functions of one leaf -------------------------------
+# On the GPU by their entry points. On the CPU those would take the eager
+# path; there the nodes are called themselves, over stand-ins of the kernels
+# that compute nothing: what is tested is what the nodes are to autograd.
+
+@pytest.fixture
+def stand_ins():
+    """The table of the kernels, its launches (csrc/hip/kernel_api.h)
+    replaced by functions that return success."""
+    hip_so = pytest.importorskip("kungfu_amd._hip")
+    pytest.importorskip("kungfu_amd._nodes")
+    where = ctypes.pythonapi.PyCapsule_GetPointer
+    where.restype = ctypes.c_void_p
+    where.argtypes = [ctypes.py_object, ctypes.c_char_p]
+    table = (ctypes.c_void_p * 9).from_address(
+        where(hip_so.kernels, b"kungfu_amd.kernels"))
+    kept = list(table)
+    done = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: 0)
+    for i in LAUNCHES:
+        table[i] = ctypes.cast(done, ctypes.c_void_p).value
+    yield table
+    table[:] = kept
+
+
+LAUNCHES = [2, 3, 5, 7, 8]  # embedding, its gradient, norm, attention, its
+
+
+def on_cpu(name, x):
+    """The node `name` as a function of x, in f32 or what it takes."""
+    if name == "embedding":
+        return hip.nodes().embedding(torch.tensor([1, 3, 3]), x, 2.0, -1,
+                                     x.dtype, 0)
+    if name == "qk_norm_rope":
+        return hip.nodes().qk_norm_rope(x, x, None, None, None, None, 0,
+                                        1e-6, 0)[0]
+    return hip.nodes().window_attention(x, x, x, None, None, 4, 0, True, 1.0,
+                                        0)
+
+
+def on_gpu(name, x):
+    if name == "embedding":
+        return embedding(torch.tensor([1, 3, 3], device="cuda"), x, 2.0)
+    if name == "qk_norm_rope":
+        return qk_norm_rope(x, x)[0]
+    return window_attention(x, x, x, window=4)
+
+
+def leaf(name, device):
+    gen = torch.Generator().manual_seed(32)
+    shape = (5, 32) if name == "embedding" else (1, 6, 2, 32)
+    dtype = BF16 if name == "window_attention" else FP32
+    return randn(gen, shape, dtype, device).requires_grad_(True)
+
+
+OPERATORS = ["embedding", "qk_norm_rope", "window_attention"]
+
+
+# ---- second derivatives ---------------------------------------------------
+
+def second_derivative(name, op, device):
+    """A term that goes through the operator's gradient next to one that
+    goes past it: no way of differentiating may drop the first."""
+    x = leaf(name, device)
+    beside = leaf(name, device)
+
+    def loss():
+        y = op(name, x)
+        g, = torch.autograd.grad((y * beside.sum()).square().sum(), x,
+                                 create_graph=True)
+        return g.square().sum() + x.square().sum() + beside.square().sum()
+
+    for t in (x, beside):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(loss(), t)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            loss().backward(inputs=[t])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        loss().backward()
+    # a graph that is made and not used does no harm
+    other = leaf(name, device)
+    got, = torch.autograd.grad(loss() + other.square().sum(), other)
+    assert torch.equal(got, 2 * other.detach())
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_second_derivative_of_a_node(name, stand_ins):
+    second_derivative(name, on_cpu, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("name", OPERATORS)
+def test_second_derivative(name):
+    second_derivative(name, on_gpu, "cuda")
+
+
+@gpu
+def test_embedding_gradient_of_a_constant_has_no_derivative():
+    """The gradient does not depend on the weight where the output's does
+    not: what is beside it is differentiated as ever."""
+    w = leaf("embedding", "cuda")
+    g, = torch.autograd.grad(on_gpu("embedding", w).sum(), w,
+                             create_graph=True)
+    got, = torch.autograd.grad(g.sum() + w.square().sum(), w)
+    assert torch.equal(got, 2 * w.detach())
 
 
 # ---- positions outside the table ------------------------------------------
