@@ -111,6 +111,16 @@ variable_list once(variable_list grads, const variable_list &from)
     return grads;
 }
 
+// There are no forward-mode derivatives: an input that has a tangent is
+// refused, as its output would have none.
+void no_tangents(const char *what, const variable_list &ts)
+{
+    for (const auto &t : ts)
+        if (t.defined() && t._fw_grad(0).defined())
+            throw std::runtime_error(
+                std::string(what) + " has no forward-mode derivative");
+}
+
 bool wants_grad(std::initializer_list<Tensor> ts)
 {
     if (!at::GradMode::is_enabled()) return false;
@@ -162,6 +172,7 @@ struct Embedding : Function<Embedding> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        no_tangents("embedding backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         auto &d = ctx->saved_data;
         const Tensor ids = ctx->get_saved_variables()[0];
@@ -190,6 +201,7 @@ struct Embedding : Function<Embedding> {
 Tensor embedding(const Tensor &ids, const Tensor &weight, double scale,
                  int64_t padding, at::ScalarType out, int64_t stream)
 {
+    no_tangents("embedding", {weight});
     const EmbedArgs a = {scale, padding, stream, out};
     if (wants_grad({weight})) return Embedding::apply(ids, weight, a);
     return embed_forward(ids, weight, a);
@@ -270,6 +282,7 @@ struct QKNormRope : Function<QKNormRope> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        no_tangents("qk_norm_rope backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &qw = s[2], &kw = s[3];
@@ -302,6 +315,8 @@ std::pair<Tensor, Tensor> qk_norm_rope(const Tensor &q, const Tensor &k,
                                        const Maybe &positions, int64_t start,
                                        double eps, int64_t stream)
 {
+    no_tangents("qk_norm_rope",
+                {q, k, or_none(qw), or_none(kw), or_none(rope)});
     const QKArgs a = {start, stream, eps};
     const auto out =
         wants_grad({q, k, or_none(qw), or_none(kw)})
@@ -381,6 +396,7 @@ struct WindowAttention : Function<WindowAttention> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        no_tangents("window_attention backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
@@ -415,6 +431,7 @@ Tensor window_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
                         int64_t window, int64_t sinks, bool causal,
                         double scale, int64_t stream)
 {
+    no_tangents("window_attention", {q_, k_, v_});
     // copies, where there are any, are part of the autograd graph
     const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
     const AttnArgs a = {window, sinks, causal, stream, scale};

@@ -125,6 +125,40 @@ def test_embedding_gradient_of_a_constant_has_no_derivative():
     assert torch.equal(got, 2 * w.detach())
 
 
+# ---- forward-mode derivatives ---------------------------------------------
+
+def forward_mode(name, op, device):
+    """Refused, of the inputs and of the gradients that come in: an output
+    without a tangent would be a derivative of zero."""
+    x = leaf(name, device)
+    y = op(name, x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(
+            x.detach(), torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            op(name, dual)
+        dy = torch.autograd.forward_ad.make_dual(
+            torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, dy)
+    for transform in (lambda f: torch.func.jvp(f, (x.detach(),),
+                                               (torch.ones_like(x),)),
+                      lambda f: torch.func.vmap(f)(x.detach()[None])):
+        with pytest.raises(RuntimeError):
+            transform(lambda t: op(name, t))
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_forward_mode_of_a_node(name, stand_ins):
+    forward_mode(name, on_cpu, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("name", OPERATORS)
+def test_forward_mode(name):
+    forward_mode(name, on_gpu, "cuda")
+
+
 # ---- positions outside the table ------------------------------------------
 
 @gpu
