@@ -9,8 +9,10 @@
 //
 // A node runs on the device and stream that its forward ran on, as the
 // engine arranges, so the stream's handle is kept from there.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -111,14 +113,20 @@ variable_list once(variable_list grads, const variable_list &from)
     return grads;
 }
 
-// There are no forward-mode derivatives: an input that has a tangent is
-// refused, as its output would have none.
-void no_tangents(const char *what, const variable_list &ts)
+// Refuses the calls whose results would be wrong without a word: of inputs
+// that have a tangent, since there are no forward-mode derivatives, and
+// those that a tracer records, since it would see the outputs' allocation
+// and not the launch that fills them.
+void usable(const char *what, const variable_list &ts)
 {
     for (const auto &t : ts)
         if (t.defined() && t._fw_grad(0).defined())
             throw std::runtime_error(
                 std::string(what) + " has no forward-mode derivative");
+    if (torch::jit::tracer::isTracing() ||
+        c10::impl::TorchDispatchModeTLS::get_mode(
+            c10::impl::TorchDispatchModeKey::PROXY))
+        throw std::runtime_error(std::string(what) + " cannot be traced");
 }
 
 bool wants_grad(std::initializer_list<Tensor> ts)
@@ -172,7 +180,7 @@ struct Embedding : Function<Embedding> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
-        no_tangents("embedding backward", grads);
+        usable("embedding backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         auto &d = ctx->saved_data;
         const Tensor ids = ctx->get_saved_variables()[0];
@@ -201,7 +209,7 @@ struct Embedding : Function<Embedding> {
 Tensor embedding(const Tensor &ids, const Tensor &weight, double scale,
                  int64_t padding, at::ScalarType out, int64_t stream)
 {
-    no_tangents("embedding", {weight});
+    usable("embedding", {weight});
     const EmbedArgs a = {scale, padding, stream, out};
     if (wants_grad({weight})) return Embedding::apply(ids, weight, a);
     return embed_forward(ids, weight, a);
@@ -282,7 +290,7 @@ struct QKNormRope : Function<QKNormRope> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
-        no_tangents("qk_norm_rope backward", grads);
+        usable("qk_norm_rope backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &qw = s[2], &kw = s[3];
@@ -315,8 +323,8 @@ std::pair<Tensor, Tensor> qk_norm_rope(const Tensor &q, const Tensor &k,
                                        const Maybe &positions, int64_t start,
                                        double eps, int64_t stream)
 {
-    no_tangents("qk_norm_rope",
-                {q, k, or_none(qw), or_none(kw), or_none(rope)});
+    usable("qk_norm_rope",
+           {q, k, or_none(qw), or_none(kw), or_none(rope)});
     const QKArgs a = {start, stream, eps};
     const auto out =
         wants_grad({q, k, or_none(qw), or_none(kw)})
@@ -396,7 +404,7 @@ struct WindowAttention : Function<WindowAttention> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
-        no_tangents("window_attention backward", grads);
+        usable("window_attention backward", grads);
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
@@ -431,7 +439,7 @@ Tensor window_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
                         int64_t window, int64_t sinks, bool causal,
                         double scale, int64_t stream)
 {
-    no_tangents("window_attention", {q_, k_, v_});
+    usable("window_attention", {q_, k_, v_});
     // copies, where there are any, are part of the autograd graph
     const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
     const AttnArgs a = {window, sinks, causal, stream, scale};

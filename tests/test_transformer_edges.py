@@ -1,10 +1,11 @@
 """Calls of the transformer operators at the edge of what they are for:
-derivatives that they do not have, rows at positions outside the table."""
+derivatives and traces that they do not have, rows at positions outside the table."""
 import ctypes
 import math
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from kungfu_amd.ops import hip
 from kungfu_amd.ops.fused_embedding import embedding
@@ -157,6 +158,42 @@ def test_forward_mode_of_a_node(name, stand_ins):
 @pytest.mark.parametrize("name", OPERATORS)
 def test_forward_mode(name):
     forward_mode(name, on_gpu, "cuda")
+
+
+# ---- tracers --------------------------------------------------------------
+
+def tracers(name, op, device):
+    """Refused: a trace would hold the output's allocation, and not what
+    fills it."""
+    x = leaf(name, device)
+    y = op(name, x)
+    dy = torch.ones_like(y)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: op(name, t), (x.detach(),),
+                        check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda t: op(name, t))(x.detach())
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda t: torch.autograd.grad(y, x, t)[0])(dy)
+    # a program that is compiled runs it as it is
+    torch._dynamo.reset()
+    run = torch.compile(lambda t: op(name, t * 1.0) + 0.0, backend="eager")
+    assert run(x.detach()).shape == y.shape
+    return run(x.detach()), y
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", OPERATORS)
+def test_tracers_of_a_node(name, stand_ins):
+    tracers(name, on_cpu, "cpu")
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", OPERATORS)
+def test_tracers(name):
+    got, want = tracers(name, on_gpu, "cuda")
+    assert torch.equal(got, want)
 
 
 # ---- positions outside the table ------------------------------------------
