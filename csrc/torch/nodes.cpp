@@ -181,9 +181,10 @@ struct Embedding : Function<Embedding> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         usable("embedding backward", grads);
+        // before autograd is off: a checkpoint computes them again here
+        const Tensor ids = ctx->get_saved_variables()[0];
         at::AutoDispatchBelowADInplaceOrView below;
         auto &d = ctx->saved_data;
-        const Tensor ids = ctx->get_saved_variables()[0];
         const auto type = (at::ScalarType)d["type"].toInt();
         const auto otype = (at::ScalarType)d["out"].toInt();
         const int64_t V = d["V"].toInt(), H = d["H"].toInt();
@@ -291,8 +292,8 @@ struct QKNormRope : Function<QKNormRope> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         usable("qk_norm_rope backward", grads);
+        const auto s = ctx->get_saved_variables();  // with autograd on
         at::AutoDispatchBelowADInplaceOrView below;
-        const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &qw = s[2], &kw = s[3];
         auto &d = ctx->saved_data;
         const QKArgs a = {d["start"].toInt(), d["stream"].toInt(),
@@ -405,8 +406,8 @@ struct WindowAttention : Function<WindowAttention> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         usable("window_attention backward", grads);
+        const auto s = ctx->get_saved_variables();  // with autograd on
         at::AutoDispatchBelowADInplaceOrView below;
-        const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
         auto &d = ctx->saved_data;
         const AttnArgs a = {d["window"].toInt(), d["sinks"].toInt(),

@@ -1,11 +1,13 @@
 """Calls of the transformer operators at the edge of what they are for:
-derivatives and traces that they do not have, rows at positions outside the table."""
+derivatives and traces that they do not have, checkpoints, rows at
+positions outside the table."""
 import ctypes
 import math
 
 import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.checkpoint import checkpoint
 
 from kungfu_amd.ops import hip
 from kungfu_amd.ops.fused_embedding import embedding
@@ -194,6 +196,36 @@ def test_tracers_of_a_node(name, stand_ins):
 def test_tracers(name):
     got, want = tracers(name, on_gpu, "cuda")
     assert torch.equal(got, want)
+
+
+# ---- checkpoints ----------------------------------------------------------
+
+def checkpointed(name, op, device):
+    """A region that ends in the operator: its inputs are computed again
+    while its backward asks for them."""
+    x = leaf(name, device)
+
+    def region(t):
+        return op(name, (t * 2.0).square())
+
+    for reentrant in (False, True):
+        y = checkpoint(region, x, use_reentrant=reentrant)
+        y.backward(torch.ones_like(y))
+        dx, x.grad = x.grad, None
+        yield dx, torch.autograd.grad(region(x), x, torch.ones_like(y))[0]
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_checkpoint_of_a_node(name, stand_ins):
+    for got, want in checkpointed(name, on_cpu, "cpu"):
+        assert got.shape == want.shape
+
+
+@gpu
+@pytest.mark.parametrize("name", OPERATORS)
+def test_checkpoint(name):
+    for got, want in checkpointed(name, on_gpu, "cuda"):
+        assert torch.equal(got, want)
 
 
 # ---- positions outside the table ------------------------------------------
