@@ -57,6 +57,9 @@ def _check(q, k, weights, rope, positions, start):
                 rope.dtype != torch.float32 or rope.device != q.device:
             raise ValueError("rope must be (positions, %d) float32 on %s" %
                              (D, q.device))
+        if rope.requires_grad and torch.is_grad_enabled():
+            raise ValueError("rope is a table of constants and gets no "
+                             "gradient")
         if positions is not None:
             hip.check_ints("positions", positions, [(S,), (B, S)], q.device)
         elif start < 0 or start + S > rope.shape[0]:
@@ -109,6 +112,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, rope=None,
     one. Where there is a table (`rope_table`), the pairs (i, i + width/2)
     are then turned by the angles of the row's position: `positions`,
     (length,) or (batch, length) int32 or int64, else start, start + 1, ...
+    The table has no gradient, and one that asks for it is refused.
 
     The width is even and at most 512. Without `positions` the range is
     checked here. A position in `positions` outside the table raises on the

@@ -228,6 +228,20 @@ def test_checkpoint(name):
         assert torch.equal(got, want)
 
 
+# ---- what has no gradient -------------------------------------------------
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_table_that_wants_a_gradient_is_refused(device):
+    q = torch.randn(1, 4, 2, 32, device=device)
+    rope = rope_table(4, 32, device=device).requires_grad_(True)
+    for x in (q, q.clone().requires_grad_(True)):
+        with pytest.raises(ValueError, match="gradient"):
+            qk_norm_rope(x, x, rope=rope)
+    with torch.no_grad():
+        assert torch.equal(qk_norm_rope(q, q, rope=rope)[0],
+                           qk_norm_rope(q, q, rope=rope.detach())[0])
+
+
 # ---- positions outside the table ------------------------------------------
 
 @gpu
