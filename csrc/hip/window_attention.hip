@@ -998,6 +998,14 @@ __device__ inline int parts_of(const Args &a, const KeyRows &k, int k0,
     return n < k.parts ? (int)n : k.parts;
 }
 
+// Blocks of f32 sums of a head: the parts of first tokens' blocks, and of the
+// others where those are cut.
+__host__ __device__ inline int kv_slots(const Args &a)
+{
+    return a.sink_blocks * a.sink_splits +
+           (a.splits > 1 ? (a.blocks - a.sink_blocks) * a.splits : 0);
+}
+
 // What dk and dv need of a tile's rows.
 template <int KT>
 struct RowData {
@@ -1022,8 +1030,6 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     __shared__ RowData rd0, rd1;
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int units =
-        a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
     const int heads = a.B * a.Hk;
     int u = blockIdx.x / heads, blk, part;
     const int bh = blockIdx.x - u * heads, slot = u;
@@ -1215,7 +1221,8 @@ __launch_bounds__(NW *WAVE, DP > 64 ? 2 : 3) void attn_dkv(const Args a)
     if (kr.parts > 1) {
         if (key >= a.T || part >= parts_of(a, kr, k0, w0)) return;
         const long long at =
-            (((long long)bh * units + slot) * NW * 32 + (key - k0)) * DP;
+            (((long long)bh * kv_slots(a) + slot) * NW * 32 + (key - k0)) *
+            DP;
         store_sums<DP>(a.part_k + at, dk, lane);
         store_sums<DP>(a.part_v + at, dv, lane);
         return;
@@ -1240,8 +1247,6 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
     __shared__ f32x4 sums[4][2][WAVE];
     const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
     const int each = a.keys * PER / WAVE;  // workgroups of a block of keys
-    const int units =
-        a.sink_blocks * a.sink_splits + (a.blocks - a.sink_blocks) * a.splits;
     const int id = blockIdx.x / each, bh = id / blocks;
     const int blk = id - bh * blocks, k0 = blk * a.keys;
     const int e = (blockIdx.x - id * each) * WAVE + lane;
@@ -1256,7 +1261,7 @@ __global__ __launch_bounds__(256) void attn_join_kv(const Args a, int blocks)
             : (long long)a.sink_blocks * a.sink_splits +
                   (long long)(blk - a.sink_blocks) * a.splits;
     const long long part = (long long)a.keys * DP;
-    const long long from = ((long long)bh * units + slot) * part + e * 4;
+    const long long from = ((long long)bh * kv_slots(a) + slot) * part + e * 4;
     f32x4 x = {}, y = {};
     const int p1 = parts * (wid + 1) / 4;
 #pragma unroll 8
@@ -1348,7 +1353,9 @@ RowPlan plan_rows(const Args &a, bool few)
 // uncut, 1131 us in halves). Where causal blocks of all lengths leave most
 // places idle behind the longest, they are cut in thirds of a share (b2
 // s4096, 16/4 heads of 128: 555 us in shares, 450 us in thirds), though the
-// sums then take more of the memory's time (38 us there).
+// sums then take more of the memory's time (38 us there). Blocks are cut only
+// where they are fewer than the places, so the parts are at most seven a
+// place, whatever the lengths: 470 MB of f32 sums.
 // The blocks with first tokens, which every row sees, are cut into eighths
 // of the others' rows, so that they fill up what those leave at the end:
 // 8192 tokens, 32/8 heads of 128, window 1024, has 504 blocks and 57 such
@@ -1386,11 +1393,15 @@ void plan_dkv(Args &a)
     a.sink_rows = a.splits_rows;
     a.sink_splits = 1;
     if (sink) {
-        // their f32 sums take 1024 x 128 keys at most
-        const long long most = 4 * CUS / (bh * sink) + 1;
+        // no more than 1024 parts in all, or one each: their f32 sums take
+        // 134 MB at most, however small the other blocks' pieces are (131072
+        // tokens, 32/8 heads of 128, window 128, 1024 first tokens: 5.4 GB
+        // if their pieces were cut as small)
+        const long long most =
+            bh * sink < 4 * CUS ? 4 * CUS / (bh * sink) : 1;
         long long n = tiles(rows / 8);
-        if (n * most < SG) n = tiles(SG / most + 1);
         if (n > piece) n = piece;
+        if (n * most < SG) n = tiles((SG + most - 1) / most);
         a.sink_rows = (int)n;
         a.sink_splits = (int)((SG + n - 1) / n);
     }
@@ -1526,7 +1537,7 @@ long long kf_attn_ws(const long long *dims, int backward)
     const RowPlan p = plan_rows(a, false);
     if (p.splits > 1) n += rows * p.splits * DP * 4;
     if (kv_parts(a))
-        n += 2ll * a.B * a.Hk * kv_units(a) * a.keys * DP * 4;
+        n += 2ll * a.B * a.Hk * kv_slots(a) * a.keys * DP * 4;
     return n;
 }
 
@@ -1612,7 +1623,7 @@ hipError_t kf_attn_bwd(const uintptr_t *ptrs, const long long *dims,
     const RowPlan p = plan_rows(a, false);
     a.part_o = a.delta + (rows * 4 + 255) / 256 * 64;
     a.part_k = a.part_o + (p.splits > 1 ? rows * p.splits * DP : 0);
-    a.part_v = a.part_k + (long long)a.B * a.Hk * kv_units(a) * a.keys * DP;
+    a.part_v = a.part_k + (long long)a.B * a.Hk * kv_slots(a) * a.keys * DP;
     hipStream_t s = (hipStream_t)stream;
 #define CASE(N)                                                             \
     if (DP == N)                                                            \

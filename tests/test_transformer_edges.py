@@ -1,6 +1,6 @@
 """Calls of the transformer operators at the edge of what they are for:
 derivatives and traces that they do not have, checkpoints, rows at
-positions outside the table."""
+positions outside the table, plans of unusual sizes."""
 import ctypes
 import math
 
@@ -13,6 +13,7 @@ from kungfu_amd.ops import hip
 from kungfu_amd.ops.fused_embedding import embedding
 from kungfu_amd.ops.qk_norm_rope import qk_norm_rope, rope_table
 from kungfu_amd.ops.window_attention import window_attention
+from test_transformer_ops import attn_check
 
 gpu = pytest.mark.gpu
 BF16, F16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -240,6 +241,50 @@ def test_a_table_that_wants_a_gradient_is_refused(device):
     with torch.no_grad():
         assert torch.equal(qk_norm_rope(q, q, rope=rope)[0],
                            qk_norm_rope(q, q, rope=rope.detach())[0])
+
+
+# ---- how attention's backward is cut ---------------------------------------
+
+def backward_workspace(B, S, T, Hk, G, D, window, sinks, causal):
+    hip_so = pytest.importorskip("kungfu_amd._hip")
+    size = ctypes.CDLL(hip_so.__file__).kf_attn_ws
+    size.restype = ctypes.c_longlong
+    return size((ctypes.c_longlong * 9)(
+        B, S, T, Hk, G, D, window or 1 << 30, sinks, causal), 1)
+
+
+def test_workspace_of_the_backward():
+    """Beside a value for each row, bounded whatever the sizes: 1024 parts
+    of first tokens' blocks and seven parts a place of the others, two f32
+    sums of 128 x 128 each, for 512 places; and 1.5 times the places of 128
+    rows for dq (at 64 columns, 768 places of half the size)."""
+    most = (1024 + 7 * 512) * 2 * 128 * 128 * 4 + 768 * 128 * 128 * 4
+    for B, Hk in ((1, 1), (1, 8), (2, 4), (4, 16), (32, 12), (7, 37)):
+        for G in (1, 4, 32):
+            for T in (1, 129, 1000, 4096, 8192, 50000, 131072, 1 << 20):
+                for window in (None, 1, 64, 128, 600, 4096):
+                    for sinks in (0, 1, 4, 200, 1024, 100000):
+                        for D in (32, 64, 128):
+                            for causal in (0, 1):
+                                size = backward_workspace(
+                                    B, T, T, Hk, G, D, window, sinks, causal)
+                                assert 0 < size <= most + 256 + \
+                                    4 * B * T * Hk * G, (
+                                        B, Hk, G, T, window, sinks, D,
+                                        causal)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,T,Hq,Hk,D,window,sinks", [
+    (4, 600, 16, 16, 64, 30, 590),   # first tokens' blocks whole
+    (1, 1000, 24, 8, 64, 40, 900),   # in fewer parts than the rows ask for
+    (1, 600, 16, 16, 64, 30, 590),   # in as many
+    (2, 900, 8, 4, 128, 100, 700)])
+def test_many_first_tokens(B, T, Hq, Hk, D, window, sinks, causal):
+    gen = torch.Generator().manual_seed(33)
+    q, k, v = (randn(gen, (B, T, h, D), BF16, "cuda") for h in (Hq, Hk, Hk))
+    attn_check(q, k, v, window, sinks, causal)
 
 
 # ---- positions outside the table ------------------------------------------
