@@ -111,13 +111,10 @@ class Bert(nn.Module):
                 nn.init.normal_(m.weight, std=0.02)
 
     def _lookup(self, table, ids, low):
-        if not self.fused_embed:
+        if not (self.fused_embed and low):
             return table(ids)
-        from kungfu_amd.ops.fused_embedding import embedding
-
         # in the activations' type: no cast of the rows after it
-        return embedding(ids, table.weight,
-                         out_dtype=torch.bfloat16 if low else None)
+        return table(ids, out_dtype=torch.bfloat16)
 
     def _embed(self, ids):
         low = self.fused_ln and ids.is_cuda

@@ -86,6 +86,7 @@ class FusedEmbedding(torch.nn.Embedding):
         self.scale = scale
         self.out_dtype = out_dtype
 
-    def forward(self, ids):
+    def forward(self, ids, out_dtype=None):
+        """`out_dtype`: of this call, where it is not the module's."""
         return embedding(ids, self.weight, self.scale, self.padding_idx,
-                         self.out_dtype)
+                         out_dtype or self.out_dtype)

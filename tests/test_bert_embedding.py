@@ -1,0 +1,38 @@
+"""BERT's embedding where `fused_embed` is set: it goes through its modules."""
+import pytest
+import torch
+
+from kungfu_amd.models.bert import Bert
+
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def make(seed, **options):
+    torch.manual_seed(seed)
+    return Bert(vocab=97, hidden=128, layers=1, heads=2, ffn=160, max_len=64,
+                fused_embed=True, **options)
+
+
+def ids_of(b, s, device):
+    gen = torch.Generator().manual_seed(1)
+    return torch.randint(0, 97, (b, s), generator=gen).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rotary", [False, True])
+@pytest.mark.parametrize("fused_ln", [False, True])
+def test_hooks_and_settings_of_the_modules(device, rotary, fused_ln):
+    m = make(1, qk_norm=rotary, rotary=rotary, fused_ln=fused_ln).to(device)
+    x, ran = ids_of(2, 9, device), []
+    tables = [t for t in (m.tok, m.pos) if t is not None]
+    for t in tables:
+        t.register_forward_hook(lambda t, args, out: ran.append(t))
+    plain = m._embed(x)
+    assert ran == tables
+    # the scale of the module is its own: none leaves the positions alone
+    m.tok.scale = 0.0
+    bare = m._embed(x)
+    assert not torch.equal(bare, plain)
+    if not rotary:
+        assert torch.equal(bare[0], bare[1])
