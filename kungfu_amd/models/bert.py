@@ -110,22 +110,20 @@ class Bert(nn.Module):
             elif isinstance(m, nn.Embedding):
                 nn.init.normal_(m.weight, std=0.02)
 
-    def _lookup(self, table, ids, low):
-        if not (self.fused_embed and low):
-            return table(ids)
-        # in the activations' type: no cast of the rows after it
-        return table(ids, out_dtype=torch.bfloat16)
-
     def _embed(self, ids):
         low = self.fused_ln and ids.is_cuda
-        x = self._lookup(self.tok, ids, low)
+        if low and self.fused_embed and self.pos is None:
+            # in the activations' type: no cast of the rows after it
+            x = self.tok(ids, out_dtype=torch.bfloat16)
+        else:  # rows that are added are rounded after that, once
+            x = self.tok(ids)
         if self.pos is not None:
             if self.fused_embed and ids.shape[1] > self.pos.num_embeddings:
                 # the lookup on the GPU would answer NaN
                 raise IndexError("%d tokens for %d positions" %
                                  (ids.shape[1], self.pos.num_embeddings))
             pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
-            x = x + self._lookup(self.pos, pos, low)
+            x = x + self.pos(pos)
         if low:
             x = x.to(torch.bfloat16)  # embeddings stay fp32 under autocast
         return self.ln(x)

@@ -36,3 +36,19 @@ def test_hooks_and_settings_of_the_modules(device, rotary, fused_ln):
     assert not torch.equal(bare, plain)
     if not rotary:
         assert torch.equal(bare[0], bare[1])
+
+
+@gpu
+@pytest.mark.parametrize("rotary", [False, True])
+def test_rows_are_rounded_once(rotary):
+    """What the first norm reads is the sum of f32 rows, rounded to bf16:
+    the same bits as without the option."""
+    m = make(2, qk_norm=rotary, rotary=rotary, fused_ln=True).cuda()
+    x, read = ids_of(2, 50, "cuda"), []
+    m.ln.register_forward_pre_hook(lambda ln, args: read.append(args[0]))
+    m._embed(x)
+    want = m.tok.weight[x]
+    if not rotary:
+        want = want + m.pos.weight[:50]
+    assert read[0].dtype == torch.bfloat16
+    assert torch.equal(read[0], want.bfloat16())
