@@ -132,8 +132,10 @@ def window_attention(q, k, v, window=None, sinks=0, causal=True,
         1.0 / math.sqrt(max(1, q.shape[-1]))
     _check(q, k, v, window, sinks, lengths, starts, scale)
     if not q.is_cuda:
-        return _eager(q, k, v, window, sinks, causal, lengths, starts,
-                      scale).to(q.dtype)
+        # the products too are of wide operands, also under autocast
+        with torch.autocast("cpu", enabled=False):
+            return _eager(q, k, v, window, sinks, causal, lengths, starts,
+                          scale).to(q.dtype)
     if 0 in q.shape or 0 in k.shape:
         # no row, or none that sees anything
         every = torch.ones((), dtype=torch.bool, device=q.device)

@@ -287,6 +287,26 @@ def test_many_first_tokens(B, T, Hq, Hk, D, window, sinks, causal):
     attn_check(q, k, v, window, sinks, causal)
 
 
+# ---- autocast on the CPU --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_eager_attention_under_autocast(dtype):
+    """Scores, softmax and sums stay in 32 bits: the same values and
+    gradients as without autocast."""
+    gen = torch.Generator().manual_seed(34)
+    leaves = [randn(gen, (2, 40, h, 32), dtype, "cpu").requires_grad_(True)
+              for h in (4, 2, 2)]
+
+    def step(on):
+        with torch.autocast("cpu", dtype=BF16, enabled=on):
+            out = window_attention(*leaves, window=9, sinks=1)
+        return (out,) + torch.autograd.grad(out, leaves,
+                                            torch.ones_like(out))
+
+    for a, b in zip(step(True), step(False)):
+        assert a.dtype == dtype and torch.equal(a, b)
+
+
 # ---- positions outside the table ------------------------------------------
 
 @gpu
