@@ -463,7 +463,9 @@ PYBIND11_MODULE(_nodes, m)
     K = (const kf_kernels *)PyCapsule_GetPointer(c.ptr(),
                                                  KF_KERNELS_CAPSULE);
     if (!K) throw py::error_already_set();
-    m.def("embedding", &embedding);
-    m.def("qk_norm_rope", &qk_norm_rope);
-    m.def("window_attention", &window_attention);
+    // other threads of the interpreter go on while memory is waited for
+    typedef py::call_guard<py::gil_scoped_release> Released;
+    m.def("embedding", &embedding, Released());
+    m.def("qk_norm_rope", &qk_norm_rope, Released());
+    m.def("window_attention", &window_attention, Released());
 }

@@ -80,6 +80,23 @@ def leaf(name, device):
 OPERATORS = ["embedding", "qk_norm_rope", "window_attention"]
 
 
+# ---- the interpreter's lock -----------------------------------------------
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_launches_do_not_hold_the_interpreter(name, grad, stand_ins):
+    """In place of the launches, the function that says whether its thread
+    holds the lock: 1, which is an error code here, if it does."""
+    holds = ctypes.cast(ctypes.pythonapi.PyGILState_Check, ctypes.c_void_p)
+    for i in LAUNCHES:
+        stand_ins[i] = holds.value
+    x = leaf(name, "cpu")
+    with torch.set_grad_enabled(grad):
+        y = on_cpu(name, x)
+    if grad:
+        torch.autograd.grad(y, x, torch.ones_like(y))
+
+
 # ---- second derivatives ---------------------------------------------------
 
 def second_derivative(name, op, device):
