@@ -69,6 +69,11 @@ Tensor dense_like(const Tensor &t)
     return at::empty(t.sizes(), t.options());
 }
 
+Tensor contiguous(const Tensor &t)
+{
+    return t.defined() ? t.contiguous() : t;
+}
+
 // Strides of the leading dimensions; 0 where the size is 1, whose stride
 // is arbitrary and never used.
 void row_strides(const Tensor &t, std::vector<long long> &to)
@@ -182,7 +187,7 @@ struct Embedding : Function<Embedding> {
     {
         usable("embedding backward", grads);
         // before autograd is off: a checkpoint computes them again here
-        const Tensor ids = ctx->get_saved_variables()[0];
+        const Tensor ids = ctx->get_saved_variables()[0].contiguous();
         at::AutoDispatchBelowADInplaceOrView below;
         auto &d = ctx->saved_data;
         const auto type = (at::ScalarType)d["type"].toInt();
@@ -294,7 +299,9 @@ struct QKNormRope : Function<QKNormRope> {
         usable("qk_norm_rope backward", grads);
         const auto s = ctx->get_saved_variables();  // with autograd on
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor &q = s[0], &k = s[1], &qw = s[2], &kw = s[3];
+        // hooks of kept tensors may give them back in another layout
+        const Tensor q = dense_rows(s[0]), k = dense_rows(s[1]);
+        const Tensor qw = contiguous(s[2]), kw = contiguous(s[3]);
         auto &d = ctx->saved_data;
         const QKArgs a = {d["start"].toInt(), d["stream"].toInt(),
                           d["eps"].toDouble()};
@@ -311,10 +318,10 @@ struct QKNormRope : Function<QKNormRope> {
                     {(int64_t)K->qk_ws((int)q.size(3),
                                        (int)(q.size(2) + k.size(2)))},
                     q.options().dtype(at::kFloat));
-            qk_launch(q, k, qw, kw, s[4], s[5], dq, dk, a, more);
+            qk_launch(q, k, qw, kw, contiguous(s[4]), s[5], dq, dk, a, more);
         }
         return once({dq, dk, more[2], more[3], Tensor(), Tensor(), Tensor()},
-                    {q, k, qw, kw, grads[0], grads[1]});
+                    {s[0], s[1], s[2], s[3], grads[0], grads[1]});
     }
 };
 
@@ -408,7 +415,10 @@ struct WindowAttention : Function<WindowAttention> {
         usable("window_attention backward", grads);
         const auto s = ctx->get_saved_variables();  // with autograd on
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor &q = s[0], &k = s[1], &v = s[2];
+        // hooks of kept tensors may give them back in another layout
+        const Tensor q = rows16(s[0]), k = rows16(s[1]), v = rows16(s[2]);
+        Tensor kept[5];  // lengths, starts, out, lse, rest
+        for (int i = 0; i < 5; ++i) kept[i] = contiguous(s[3 + i]);
         auto &d = ctx->saved_data;
         const AttnArgs a = {d["window"].toInt(), d["sinks"].toInt(),
                             d["causal"].toInt(), d["stream"].toInt(),
@@ -424,14 +434,15 @@ struct WindowAttention : Function<WindowAttention> {
             at::empty({(int64_t)K->attn_ws(dims.data(), 1)},
                       q.options().dtype(at::kByte));
         const uintptr_t ptrs[13] = {
-            ptr(q),    ptr(k),    ptr(v),    ptr(s[5]), ptr(s[6]),
-            ptr(s[7]), ptr(s[3]), ptr(s[4]), ptr(dout), ptr(dq),
-            ptr(dk),   ptr(dv),   ptr(ws)};
+            ptr(q),       ptr(k),       ptr(v),       ptr(kept[2]),
+            ptr(kept[3]), ptr(kept[4]), ptr(kept[0]), ptr(kept[1]),
+            ptr(dout),    ptr(dq),      ptr(dk),      ptr(dv),
+            ptr(ws)};
         check(K->attn_bwd(ptrs, dims.data(), strides.data(), (float)a.scale,
                           type_code(q.scalar_type()), (void *)a.stream),
               "window_attention backward");
         return once({dq, dk, dv, Tensor(), Tensor(), Tensor()},
-                    {q, k, v, grads[0]});
+                    {s[0], s[1], s[2], grads[0]});
     }
 };
 

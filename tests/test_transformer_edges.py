@@ -246,6 +246,39 @@ def test_checkpoint(name):
         assert torch.equal(got, want)
 
 
+# ---- kept tensors in another layout ---------------------------------------
+
+@gpu
+@pytest.mark.parametrize("name", OPERATORS)
+def test_hooks_may_change_the_layout_of_kept_tensors(name):
+    """What a hook gives back has the kept tensor's values, type and size,
+    and strides of its own; or was on the host in between."""
+    def turned(t):  # the last dimension is the widest apart
+        return t.movedim(-1, 0).contiguous().movedim(0, -1)
+
+    x = leaf(name, "cuda")
+    assert name == "embedding" or turned(x).stride(-1) != 1
+
+    def step():
+        y = on_gpu(name, x)
+        return torch.autograd.grad(y, x, torch.ones_like(y))[0]
+
+    def attend():
+        k = x.detach()
+        lengths = torch.tensor([[5, 9]], device="cuda")[:, 0]
+        y = window_attention(x, k, k, window=4, lengths=lengths)
+        return torch.autograd.grad(y, x, torch.ones_like(y))[0]
+
+    for run in (step, attend) if name == "window_attention" else (step,):
+        want = run()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned):
+            got = run()
+        assert torch.equal(got, want)
+        with torch.autograd.graph.save_on_cpu():
+            got = run()
+        assert torch.equal(got, want)
+
+
 # ---- what has no gradient -------------------------------------------------
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
