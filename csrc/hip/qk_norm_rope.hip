@@ -322,17 +322,20 @@ __global__ __launch_bounds__(BLOCK) void qk_bwd(const Args a)
             }
             const float r = rsqrtf(group_sum(q, L) / (float)a.D + a.eps);
             const float m = group_sum(t, L) / (float)a.D * r * r * r;
-            if (on[u]) {
-                // a row at a position outside the table has no gradient,
-                // whatever it holds: zeros, and no part in the weights'
+            if (on[u] && ang[u].ok) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    al[j] += ang[u].ok ? gl[j] * lo[j] * r : 0.f;
-                    ah[j] += ang[u].ok ? gh[j] * hi[j] * r : 0.f;
-                    gl[j] = ang[u].ok ? gl[j] * wl[j] * r - lo[j] * m : 0.f;
-                    gh[j] = ang[u].ok ? gh[j] * wh[j] * r - hi[j] * m : 0.f;
+                    al[j] += gl[j] * lo[j] * r;
+                    ah[j] += gh[j] * hi[j] * r;
+                    gl[j] = gl[j] * wl[j] * r - lo[j] * m;
+                    gh[j] = gh[j] * wh[j] * r - hi[j] * m;
                 }
                 store_pairs<T, VEC>(out[u], gl, gh, half, li, L);
+            } else if (on[u]) {
+                // a row at a position outside the table has no gradient,
+                // whatever it holds: zeros, and no part in the weights'
+                const float zero[8] = {};
+                store_pairs<T, VEC>(out[u], zero, zero, half, li, L);
             }
         }
     }
