@@ -55,7 +55,7 @@ HIP_ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 
-def _hipcc_ext(name, sources, out_dir, extra_link=()):
+def _hipcc_ext(name, sources, out_dir, extra_link=(), force=False):
     """Compile one hipcc extension in-tree (gfx950 only)."""
     import sysconfig
 
@@ -73,7 +73,7 @@ def _hipcc_ext(name, sources, out_dir, extra_link=()):
 
         deps = [src_path, os.path.abspath(__file__)] + glob.glob(
             os.path.join(ROOT, "csrc", "**", "*.h*"), recursive=True)
-        if (os.path.exists(obj) and
+        if (not force and os.path.exists(obj) and
                 os.path.getmtime(obj) > max(map(os.path.getmtime, deps))):
             objs.append(obj)
             continue
@@ -95,17 +95,17 @@ def _hipcc_ext(name, sources, out_dir, extra_link=()):
     return out
 
 
-def build_hip_ext(out_dir):
-    return _hipcc_ext("_hip", HIP_SOURCES, out_dir)
+def build_hip_ext(out_dir, force=False):
+    return _hipcc_ext("_hip", HIP_SOURCES, out_dir, force=force)
 
 
-def build_rccl_ext(out_dir):
-    return _hipcc_ext("_rccl", RCCL_SOURCES, out_dir,
+def build_rccl_ext(out_dir, force=False):
+    return _hipcc_ext("_rccl", RCCL_SOURCES, out_dir, force=force,
                       extra_link=["-L/opt/rocm/lib", "-lrccl",
                                   "-Wl,-rpath,/opt/rocm/lib"])
 
 
-def build_nodes_ext(out_dir):
+def build_nodes_ext(out_dir, force=False):
     """The autograd nodes, against the installed torch."""
     import sysconfig
 
@@ -117,7 +117,7 @@ def build_nodes_ext(out_dir):
                        "_nodes" + sysconfig.get_config_var("EXT_SUFFIX"))
     deps = [src, os.path.join(ROOT, "csrc", "hip", "kernel_api.h"),
             os.path.abspath(__file__)]
-    if os.path.exists(out) and \
+    if not force and os.path.exists(out) and \
             os.path.getmtime(out) > max(map(os.path.getmtime, deps)):
         return out
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -139,9 +139,9 @@ class BuildExt(build_ext):
         if os.environ.get("KUNGFU_SKIP_HIP", "0") != "1":
             if os.path.exists(HIPCC):
                 dest = os.path.join(ROOT, "kungfu_amd")
-                build_hip_ext(dest)
-                build_rccl_ext(dest)
-                build_nodes_ext(dest)
+                build_hip_ext(dest, self.force)
+                build_rccl_ext(dest, self.force)
+                build_nodes_ext(dest, self.force)
             else:
                 print("hipcc not found; skipping kungfu_amd._hip/_rccl/"
                       "_nodes")
