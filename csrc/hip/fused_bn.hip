@@ -359,6 +359,11 @@ __global__ void bn_bwd_reduce_kernel(
                     mk[j] = 0xffff;
                 }
             }
+            // all loads are on their way before one is waited for: left to
+            // itself the compiler sends the last ones after a wait for the
+            // first (27.4 us for 23.3, mean of ResNet-50's layers at 64
+            // images)
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < ILP; ++j) {
 #pragma unroll
