@@ -13,7 +13,7 @@
 //
 // Both are bound by memory: forward reads x and writes y once, backward
 // reads x and dy and writes dx once (2 x 8192 tokens, 32/8 heads of 128 in
-// bf16: 335 MB in 62 us, 5.4 TB/s, and 503 MB in 116 us, 4.3 TB/s). A row
+// bf16: 335 MB in 63 us, 5.3 TB/s, and 503 MB in 117 us, 4.3 TB/s). A row
 // is held by L = D/16 lanes (rounded up to a power of two) with eight pairs
 // each, so the rotation needs no exchange between lanes and the norm log2(L)
 // shuffles.

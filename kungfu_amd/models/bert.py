@@ -9,7 +9,8 @@ Options beside the plain encoder, each off by default: `fused_embed` (the
 lookup in the activations' type, gradient by sorted tokens), `qk_norm` and
 `rotary` (norm of queries and keys for each head, positions by rotation
 instead of an embedding), `window`/`sinks`/`causal` (attention to near and
-first tokens), and padded batches by `lengths`.
+first tokens), and padded batches by `lengths`. On the GPU all but the first
+need 16-bit activations: bf16 weights, or autocast.
 """
 import torch
 import torch.nn as nn
