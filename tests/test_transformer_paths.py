@@ -5,7 +5,8 @@ import torch
 
 from kungfu_amd.ops.fused_embedding import embedding
 from kungfu_amd.ops.qk_norm_rope import qk_norm_rope, rope_table
-from test_transformer_ops import (BF16, F16, F32, FP32, attn_check,
+from kungfu_amd.ops.window_attention import window_attention
+from test_transformer_ops import (BF16, F16, F32, FP32, attn_check, mask_of,
                                   qk_oracle, randn)
 
 gpu = pytest.mark.gpu
@@ -119,6 +120,47 @@ def test_rows_in_parts(causal, D):
     q, k, v = (randn(gen, (1, 1500, h, D), BF16, "cuda") for h in (4, 2, 2))
     attn_check(q, k, v, None, 0, causal)
     attn_check(q, k, v, None, 0, causal, lengths=[1111])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("S,D,window,sinks,causal", [
+    (130, 64, 2, 0, False), (700, 128, 9, 4, True), (300, 32, 3, 20, False),
+    (32, 96, None, 0, False), (5, 64, None, 0, True), (200, 80, 32, 0, True)])
+def test_gradients_of_rows_that_see_few_keys(dtype, S, D, window, sinks,
+                                             causal):
+    """Values have a common offset, which gradients of the scores are free
+    of. Each of those, w (dw - sum w dw), is off by its rounding to the type
+    as an operand and by f32 errors of its parts, and not by roundings of
+    the weights that the output was summed with."""
+    gen = torch.Generator().manual_seed(45)
+    q, k, v, dout = (randn(gen, (1, S, 2, D), FP32, "cpu") for _ in range(4))
+    q, k, v, dout = (t.to(dtype).cuda() for t in (q, k, v + 16, dout))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(
+        window_attention(*leaves, window=window, sinks=sinks, causal=causal),
+        leaves[:2], dout)
+    u, scale = torch.finfo(dtype).eps / 2, D ** -0.5
+    see = mask_of(S, S, 0, S, window, sinks, causal)
+    for h in range(2):
+        a, b, c, g = (t.detach()[0, :, h].double().cpu()
+                      for t in (q, k, v, dout))
+        x = (a @ b.T * scale).masked_fill(~see, -float("inf"))
+        p, dp = torch.softmax(x, 1), g @ c.T
+        delta = (p * dp).sum(1, keepdim=True)
+        ds = p * (dp - delta)
+        # f32 scores, exponentials and sums: of D products, of S weights
+        e = 6 * (D + 8) * F32 * (1 + float(
+            (a.abs() @ b.abs().T).max() * scale)) + 2 * S * F32
+        most = (g.abs() @ c.abs().T).masked_fill(~see, 0).amax(
+            1, keepdim=True)
+        derr = (u + e) * ds.abs() + (1 + u) * p * 2 * e * most
+        for t, want, bound in (
+                (got[0], ds @ b * scale, derr @ b.abs() * scale),
+                (got[1], ds.T @ a * scale, derr.T @ a.abs() * scale)):
+            t = t[0, :, h].double().cpu()
+            over = (t - want).abs() - bound * (1 + u) - u * want.abs()
+            assert float(over.max()) < 1e-7
 
 
 @gpu
