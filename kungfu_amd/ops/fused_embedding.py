@@ -87,6 +87,6 @@ class FusedEmbedding(torch.nn.Embedding):
         self.out_dtype = out_dtype
 
     def forward(self, ids, out_dtype=None):
-        """`out_dtype`: of this call, where it is not the module's."""
+        """`out_dtype`: of this call, where the module has none of its own."""
         return embedding(ids, self.weight, self.scale, self.padding_idx,
-                         out_dtype or self.out_dtype)
+                         self.out_dtype or out_dtype)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from kungfu_amd.models.bert import Bert
+from kungfu_amd.ops.fused_embedding import FusedEmbedding
 
 gpu = pytest.mark.gpu
 DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
@@ -52,3 +53,13 @@ def test_rows_are_rounded_once(rotary):
         want = want + m.pos.weight[:50]
     assert read[0].dtype == torch.bfloat16
     assert torch.equal(read[0], want.bfloat16())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_module_keeps_its_own_type(device):
+    m = FusedEmbedding(9, 16, out_dtype=torch.float16).to(device)
+    x = torch.tensor([1, 8], device=device)
+    assert m(x, out_dtype=torch.bfloat16).dtype == torch.float16
+    m.out_dtype = None
+    assert m(x, out_dtype=torch.bfloat16).dtype == torch.bfloat16
+    assert m(x).dtype == torch.float32
